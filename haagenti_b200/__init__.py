@@ -14,6 +14,8 @@ CUDA library (libhct_b200.so) through its C ABI:
 * ``HctReader`` / ``HctReaderV2`` -- crates/haagenti-hct/src/tensor.rs:408-516,
   832-1021, with ``decompress_all`` on the GPU and ``decode`` for the full
   LZ4 -> INT4 -> IDCT pipeline.
+* ``linear`` / ``grouped_linear`` -- products with the decoded weights, dense
+  or straight from the INT4 payload (``Int4Weight``, ``HctReader.int4_weight``).
 
 Errors are raised as ``HaagentiError`` subclasses named after the
 haagenti_core::Error variants (crates/haagenti-core/src/error.rs:10-65).
@@ -26,9 +28,11 @@ import ctypes as C
 import numpy as np
 
 from . import _lib as L
-from ._lib import BF16, F16, F32, FLAG_SPECTRAL_Q4
+from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_RELU, ACT_SILU, BF16, F16, F32,
+                   FLAG_SPECTRAL_Q4)
 
 IDCT_AUTO, IDCT_DENSE, IDCT_SCATTER = 0, 1, 2
+_DTYPE_I4 = 4  # haagenti_hct::DType tag (tensor.rs:98-105)
 
 __all__ = [
     "HaagentiError", "CorruptedData", "BufferTooSmall", "UnexpectedEof", "ChecksumMismatch",
@@ -36,7 +40,8 @@ __all__ = [
     "dequantize_int4_mp", "idct_2d",
     "spectral_q4_decode", "HctReader", "HctReaderV2", "HctV3Decoder", "hct_v3_decode",
     "HoloTensorReader", "ZstdDecompressor", "ZstdGpuPipeline", "zstd_decompress", "F32",
-    "F16", "BF16", "FLAG_SPECTRAL_Q4",
+    "F16", "BF16", "FLAG_SPECTRAL_Q4", "Int4Weight", "linear", "grouped_linear", "linear_status",
+    "ACT_NONE", "ACT_RELU", "ACT_SILU", "ACT_GELU", "ACT_GELU_TANH",
 ]
 
 
@@ -687,6 +692,16 @@ class HctReader:
         _check(rc, err)
         return out
 
+    def int4_weight(self, stream=None):
+        """The tensor of a plain INT4 file (no spectral flag) as an ``Int4Weight``:
+        its payload decompressed and laid out for ``linear`` on the GPU."""
+        h = self.header()
+        if h["dtype"] != _DTYPE_I4 or h["flags"] & FLAG_SPECTRAL_Q4:
+            raise Unsupported(L.UNSUPPORTED, "int4_weight: not a plain INT4 tensor")
+        if len(h["shape"]) != 2:
+            raise Unsupported(L.UNSUPPORTED, f"int4_weight: a matrix is 2-D, got {h['shape']}")
+        return Int4Weight(self.decompress_all(stream), *h["shape"], stream=stream)
+
     def wait(self):
         """Status of the last ``decode_async`` (raises like ``decode``)."""
         err = L.Error()
@@ -711,3 +726,6 @@ class HctReaderV2(HctReader):
 
     def decompress_all_validated(self, stream=None):
         return self.decompress_all(stream)
+
+
+from .products import Int4Weight, grouped_linear, linear, linear_status  # noqa: E402

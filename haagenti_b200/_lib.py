@@ -28,6 +28,8 @@ SIZE_MISMATCH = 24
 
 F32, F16, BF16 = 0, 1, 2
 FLAG_SPECTRAL_Q4 = 0x0100
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = range(5)
+WEIGHT_DENSE, WEIGHT_INT4 = 0, 1
 
 
 class Lz4Block(C.Structure):
@@ -68,6 +70,17 @@ class Int4Job(C.Structure):
                 ("d_out", C.c_void_p)]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = [("rows", C.c_uint64), ("out_features", C.c_uint64), ("in_features", C.c_uint64),
+                ("d_x", C.c_void_p), ("ldx", C.c_uint64), ("d_weight", C.c_void_p),
+                ("ldw", C.c_uint64), ("weight_stride", C.c_uint64), ("d_bias", C.c_void_p),
+                ("d_gate", C.c_void_p), ("ldgate", C.c_uint64), ("d_residual", C.c_void_p),
+                ("ldresidual", C.c_uint64), ("d_out", C.c_void_p), ("ldout", C.c_uint64),
+                ("d_offsets", C.c_void_p), ("experts", C.c_uint32), ("offsets_bits", C.c_int32),
+                ("x_dtype", C.c_int32), ("weight_form", C.c_int32), ("bias_dtype", C.c_int32),
+                ("out_dtype", C.c_int32), ("activation", C.c_int32), ("reserved", C.c_int32)]
+
+
 class KernelStats(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("launches", C.c_uint64), ("total_ms", C.c_double),
                 ("work", C.c_double)]
@@ -105,6 +118,11 @@ SIGNATURES = {
                                               C.POINTER(C.c_size_t), _vp]),
     "hct_b200_dequantize_int4_batch": (C.c_int, [C.POINTER(Int4Job), C.c_uint32, C.c_int,
                                                  C.POINTER(C.c_size_t), _vp]),
+    "hct_b200_linear": (C.c_int, [C.POINTER(LinearArgs), _vp]),
+    "hct_b200_grouped_linear": (C.c_int, [C.POINTER(LinearArgs), _vp]),
+    "hct_b200_linear_status": (C.c_int, [_vp]),
+    "hct_b200_int4_weight_bytes": (C.c_size_t, [_sz, _sz]),
+    "hct_b200_int4_weight_pack": (C.c_int, [_vp, _sz, _sz, _sz, _vp, _vp]),
     "hct_b200_idct_2d": (C.c_int, [_vp, _vp, _vp, C.c_int, _sz, _sz, _vp]),
     "hct_b200_spectral_q4_decode": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, C.c_int, _vp]),
     "hct_b200_spectral_q4_decode_noalloc": (C.c_int, [_vp, _sz, _sz, _sz, _vp, C.c_int, _vp]),

@@ -1,0 +1,252 @@
+"""Products with decoded weights: ``linear`` and ``grouped_linear``.
+
+    y = act(x Wt + bias) * gate + residual
+
+on the GPU, one kernel launch per call and no host synchronisation.  W is a
+dense (out_features, in_features) tensor, as ``HctReader.decode`` returns it,
+or an ``Int4Weight``: the INT4 payload of a plain INT4 file
+(``HctReader.decompress_all``) laid out once for the kernels, so that the
+weights are read in 4.5 bits each.  The reference has no counterpart: it hands
+its decoded tensors to an external runtime.
+"""
+from __future__ import annotations
+
+from . import (F16, BF16, F32, Unsupported, _as_host_u8, _check, _torch)
+from . import _lib as L
+from ._lib import ACT_NONE
+
+__all__ = ["Int4Weight", "linear", "grouped_linear", "linear_status"]
+
+_TAG: dict = {}   # torch dtype -> F32 / F16 / BF16
+_TYPE: dict = {}  # and back
+
+
+def _types():
+    torch = _torch()
+    _TAG.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    _TYPE.update({v: k for k, v in _TAG.items()})
+    return _TAG
+
+
+class Int4Weight:
+    """A rows x cols matrix in ``quantize_int4`` form (one f16 scale per 32
+    values of a row; cols a multiple of 32), or a list of such matrices (one
+    per expert, for ``grouped_linear``), laid out for the products.
+
+    ``data`` is a payload: f16 scales, then nibbles, as a CUDA uint8 tensor or
+    host bytes; or a list of payloads.  The layout is made here, once, and the
+    stream is synchronised before the constructor returns, so that the weight
+    may be used on any stream of its device."""
+
+    def __init__(self, data, rows: int, cols: int, device=None, stream=None):
+        torch = _torch()
+        many = isinstance(data, (list, tuple))
+        parts = list(data) if many else [data]
+        rows, cols = int(rows), int(cols)
+        lib = L.load()
+        size = lib.hct_b200_int4_weight_bytes(rows, cols) if rows > 0 and cols > 0 else 0
+        if not size:
+            raise ValueError(f"an INT4 weight of {rows} x {cols}: cols must be a positive multiple "
+                             "of 32 and rows positive")
+        if not parts:
+            raise ValueError("an INT4 weight needs a payload")
+        for p in parts:
+            if hasattr(p, "is_cuda") and p.is_cuda:
+                if p.dtype != torch.uint8 or p.dim() != 1 or not p.is_contiguous():
+                    raise ValueError("an INT4 payload is a contiguous 1-D uint8 tensor")
+                if device is None:
+                    device = p.device
+                elif p.device != torch.device(device):
+                    raise ValueError("the payloads of one weight are on one device")
+        if device is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        device = torch.device(device)
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        with torch.cuda.device(device):
+            stream = stream if stream is not None else torch.cuda.current_stream()
+            with torch.cuda.stream(stream):
+                if torch.cuda.is_current_stream_capturing():
+                    raise Unsupported(L.UNSUPPORTED, "an INT4 weight cannot be laid out while its "
+                                                     "stream is being captured")
+                packed = torch.empty(len(parts) * size, dtype=torch.uint8, device=device)
+                for i, p in enumerate(parts):
+                    if not (hasattr(p, "is_cuda") and p.is_cuda):
+                        p = torch.from_numpy(_as_host_u8(p).copy()).to(device)
+                    _check(lib.hct_b200_int4_weight_pack(
+                        p.data_ptr(), p.numel(), rows, cols, packed.data_ptr() + i * size,
+                        stream.cuda_stream))
+                stream.synchronize()
+        self.rows, self.cols = rows, cols
+        self.experts = len(parts) if many else None
+        self.packed = packed
+        self.device = device
+
+    @property
+    def shape(self):
+        s = (self.rows, self.cols)
+        return s if self.experts is None else (self.experts,) + s
+
+
+def _matrix(t, name, shape, dtype, device):
+    """Row stride of an optional (rows, features) operand after its checks."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, x on {device}")
+    s = t.stride()
+    if s[1] != 1 and shape[1] > 1:
+        raise ValueError(f"the features of {name} must be contiguous")
+    return s[0]
+
+
+def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, out, stream):
+    torch = _torch()
+    tags = _TAG or _types()
+    if x.dim() != 2 or not x.is_cuda:
+        raise ValueError("x must be a 2-D CUDA tensor (rows, in_features)")
+    device = x.device
+    m, k = x.shape
+    xt = x.dtype
+    x_tag = tags.get(xt)
+    if x_tag is None or x_tag == F32:
+        raise ValueError(f"x must be float16 or bfloat16, got {xt}")
+    sx = x.stride()
+    if sx[1] != 1 and k > 1:
+        raise ValueError("the features of x must be contiguous")
+    ldw = w_stride = 0
+    experts = None
+    if isinstance(weight, Int4Weight):
+        form, wt = L.WEIGHT_INT4, weight.packed
+        n, wk = weight.rows, weight.cols
+        experts = weight.experts
+    else:
+        form, wt = L.WEIGHT_DENSE, weight
+        if weight.dtype != xt:
+            raise ValueError(f"a dense weight must be of x's type {xt}, got {weight.dtype}")
+        if weight.dim() != (2 if offsets is None else 3):
+            raise ValueError("a dense weight is (out_features, in_features), with a leading axis "
+                             "of experts in grouped_linear")
+        n, wk = weight.shape[-2:]
+        ws = weight.stride()
+        if ws[-1] != 1 and wk > 1:
+            raise ValueError("the input features of a dense weight must be contiguous")
+        ldw = ws[-2]
+        if offsets is not None:
+            experts, w_stride = weight.shape[0], ws[0]
+    if wk != k:
+        raise ValueError(f"x has {k} features, the weight {wk}")
+    if wt.device != device:
+        raise ValueError(f"the weight is on {wt.device}, x on {device}")
+    bits = 32
+    if offsets is None:
+        if experts is not None:
+            raise ValueError("a weight with experts needs grouped_linear")
+        experts = 0
+        off_ptr = None
+    else:
+        if experts is None:
+            raise ValueError("grouped_linear needs a weight with experts (an Int4Weight of a list)")
+        if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != device:
+            raise ValueError("offsets must be an int32 or int64 tensor on x's device")
+        if offsets.dim() != 1 or offsets.shape[0] != experts + 1 or not offsets.is_contiguous():
+            raise ValueError(f"offsets must hold experts + 1 = {experts + 1} contiguous values")
+        bits = 32 if offsets.dtype == torch.int32 else 64
+        off_ptr = offsets.data_ptr()
+    if out is not None:
+        tag = tags.get(out.dtype)
+        if tag is None or (out_dtype is not None and out_dtype != tag):
+            raise ValueError(f"out is of {out.dtype}, not of out_dtype {out_dtype}")
+    else:
+        tag = x_tag if out_dtype is None else out_dtype
+        if tag not in _TYPE:
+            raise ValueError(f"out_dtype must be F32, F16 or BF16, got {out_dtype}")
+    ot = _TYPE[tag]
+    shape = (m, n)
+    bias_tag = x_tag
+    if bias is not None:
+        want = (n,) if offsets is None else (experts, n)
+        bias_tag = tags.get(bias.dtype)
+        if (bias_tag != x_tag and bias_tag != F32) or tuple(bias.shape) != want:
+            raise ValueError(f"bias must be {want} of {xt} or float32, got {tuple(bias.shape)} of "
+                             f"{bias.dtype}")
+        if bias.device != device or not bias.is_contiguous():
+            raise ValueError("bias must be contiguous and on x's device")
+    ldg = _matrix(gate, "gate", shape, xt, device) if gate is not None else 0
+    ldr = _matrix(residual, "residual", shape, ot, device) if residual is not None else 0
+    if out is not None:
+        _matrix(out, "out", shape, ot, device)
+    if torch.is_grad_enabled():
+        for t in (x, weight, bias, gate, residual, out):
+            if t is not None and getattr(t, "requires_grad", False):
+                raise Unsupported(L.UNSUPPORTED, "the products have no backward pass: detach the "
+                                                 "tensors or call under torch.no_grad()")
+    lib = L.load()
+    fn = lib.hct_b200_linear if offsets is None else lib.hct_b200_grouped_linear
+
+    def call(raw):
+        o = out if out is not None else torch.empty(shape, dtype=ot, device=device)
+        args = L.LinearArgs(
+            m, n, k, x.data_ptr(), sx[0], wt.data_ptr(), ldw, w_stride,
+            None if bias is None else bias.data_ptr(),
+            None if gate is None else gate.data_ptr(), ldg,
+            None if residual is None else residual.data_ptr(), ldr,
+            o.data_ptr(), o.stride(0), off_ptr, experts, bits, x_tag, form, bias_tag, tag,
+            activation, 0)
+        _check(fn(args, raw))
+        return o
+
+    if stream is None and torch.cuda.current_device() == device.index:
+        return call(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        if stream is None or stream == torch.cuda.current_stream():
+            return call(torch.cuda.current_stream().cuda_stream)
+        if stream.device != device:
+            raise ValueError(f"the stream belongs to {stream.device}, x to {device}")
+        with torch.cuda.stream(stream):
+            o = call(stream.cuda_stream)
+        # the caller's tensors are read on a stream that their allocator does not know of
+        for t in (x, wt, offsets, bias, gate, residual, out):
+            if t is not None:
+                t.record_stream(stream)
+        return o
+
+
+def linear(x, weight, bias=None, activation: int = ACT_NONE, gate=None, residual=None,
+           out_dtype: int | None = None, out=None, stream=None):
+    """act(x Wt + bias) * gate + residual: (rows, out_features) of ``out_dtype``.
+
+    ``x`` is (rows, in_features) in float16 or bfloat16, with contiguous
+    features and any row stride; ``weight`` a dense tensor of x's type or an
+    ``Int4Weight``; ``bias`` (out_features,) of x's type or float32;
+    ``activation`` one of the ACT_ constants; ``gate`` (rows, out_features) of
+    x's type; ``residual`` of the output's type, which is x's by default.
+    ``out`` may be ``gate`` or ``residual`` itself.  Sums are held in f32 and
+    the result rounded once; ``out_dtype=F32`` also keeps INT4 weights exact.
+    There is no backward pass: tensors that require a gradient are refused
+    while autograd records."""
+    return _product(x, weight, None, bias, activation, gate, residual, out_dtype, out, stream)
+
+
+def grouped_linear(x, weight, offsets, bias=None, activation: int = ACT_NONE, gate=None,
+                   residual=None, out_dtype: int | None = None, out=None, stream=None):
+    """``linear`` with one weight per expert: rows [offsets[e], offsets[e+1]) of
+    ``x``, which is sorted by expert, go through expert e.
+
+    ``weight`` is a dense (experts, out_features, in_features) tensor or an
+    ``Int4Weight`` of a list; ``bias`` (experts, out_features); ``offsets``
+    experts + 1 ascending int32 or int64 values on x's device, read there (no
+    synchronisation).  Rows before offsets[0] and from offsets[-1] on are left
+    as they were in ``out`` (undefined where ``out`` is not given)."""
+    if offsets is None:
+        raise ValueError("grouped_linear needs offsets")
+    return _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, out, stream)
+
+
+def linear_status(device=None, stream=None):
+    """Synchronise and raise if a product on the device ran into a device-side
+    timeout since the last call (its output is then undefined)."""
+    torch = _torch()
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        s = stream if stream is not None else torch.cuda.current_stream()
+        _check(L.load().hct_b200_linear_status(s.cuda_stream))

@@ -232,6 +232,87 @@ int hct_b200_dequantize_int4_batch(const hct_b200_int4_job *jobs, uint32_t num_j
 int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t num_elements,
                                 void *d_out, int out_dtype, size_t *written, void *stream);
 
+/* ---- products with decoded weights ---------------------------------------
+ * What a loader's weights are for (no reference counterpart; the reference
+ * hands its tensors to an external runtime):
+ *     out[i][j] = act(sum_k x[i][k] w[j][k] + bias[j]) * gate[i][j] + residual[i][j]
+ * for i < rows, j < out_features, k < in_features, with w, like every weight
+ * this library decodes, [out, in] row-major.  w is either a dense matrix of
+ * x's type (hct_b200_reader_decode) or an INT4 payload in the quantize_int4
+ * layout (hct_b200_reader_decompress_all of a plain INT4 file), laid out once
+ * by hct_b200_int4_weight_pack.  bias, gate and residual may be NULL.
+ *
+ * grouped_linear: rows [offsets[e], offsets[e+1]) are multiplied by expert e's
+ * matrix (and bias).  offsets is read on the device, with no host
+ * synchronisation: experts + 1 ascending values.  Rows before offsets[0] and
+ * from offsets[experts] on are neither read nor written.  Values outside
+ * [0, rows] are clamped to it and a pair that descends is an empty group, so
+ * that wrong offsets give wrong rows and no access out of range.
+ *
+ * Types: x F16 or BF16, gate of x's type; bias of x's type or F32; residual
+ * of out's type; out F16, BF16 or F32.  Sums are held in f32 and the result is
+ * rounded once.  The tensor cores truncate each partial sum they add to
+ * (relative error about in_features / 16 * 2^-25), which the 16-bit outputs
+ * do not show; F32 outputs are therefore summed in sections of 256 that are
+ * added with rounding.  INT4 weights are (nibble - 8) * scale: rounded to
+ * x's type as hct_b200_dequantize_int4 rounds them for 16-bit outputs, and
+ * held exactly (as the sum of two values of x's type) for F32 outputs.
+ *
+ * Strides are in elements.  Rows of x and w that start on 16-byte boundaries
+ * take the tensor-core path; others are handled by a slower kernel.  out may
+ * be the same matrix as gate or residual (same pointer, stride and type); any
+ * other overlap of out with an input is HCT_B200_ERR_INVALID_ARGUMENT, as are
+ * out rows that overlap one another.  rows == 0 or out_features == 0 is a
+ * no-op; in_features == 0 is a product of zero.  At most 1024 experts, sizes
+ * below 2^31, row strides up to 2^30 elements.
+ * The calls allocate nothing, use no context and no shared scratch, and may be
+ * captured; they run on the calling thread's current device, to which the
+ * pointers and the stream must belong.  A device-side wait that expires is
+ * reported by hct_b200_linear_status, which synchronises `stream` and returns
+ * (and clears) the current device's status of every product since its last
+ * call: HCT_B200_OK or HCT_B200_ERR_TIMEOUT, after which the outputs are
+ * undefined. */
+enum {
+    HCT_B200_ACT_NONE = 0,
+    HCT_B200_ACT_RELU = 1,
+    HCT_B200_ACT_SILU = 2,
+    HCT_B200_ACT_GELU = 3,      /* z Phi(z), by erf */
+    HCT_B200_ACT_GELU_TANH = 4  /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+};
+enum { HCT_B200_WEIGHT_DENSE = 0, HCT_B200_WEIGHT_INT4 = 1 };
+typedef struct {
+    uint64_t rows, out_features, in_features;
+    const void *d_x;
+    uint64_t ldx;
+    const void *d_weight;      /* dense: [experts][out][in]; INT4: packed matrices, one after another */
+    uint64_t ldw;              /* dense: row stride */
+    uint64_t weight_stride;    /* dense: stride between experts (elements) */
+    const void *d_bias;        /* [experts][out], contiguous */
+    const void *d_gate;
+    uint64_t ldgate;
+    const void *d_residual;
+    uint64_t ldresidual;
+    void *d_out;
+    uint64_t ldout;
+    const void *d_offsets;     /* experts + 1 int32 or int64 (grouped_linear) */
+    uint32_t experts;
+    int32_t offsets_bits;      /* 32 or 64 */
+    int32_t x_dtype, weight_form, bias_dtype, out_dtype, activation;
+    int32_t reserved;          /* 0 */
+} hct_b200_linear_args;
+int hct_b200_linear(const hct_b200_linear_args *args, void *stream); /* d_offsets, experts unused */
+int hct_b200_grouped_linear(const hct_b200_linear_args *args, void *stream);
+int hct_b200_linear_status(void *stream);
+/* Bytes of one packed rows x cols INT4 matrix, 0 when cols is not a multiple
+ * of 32 (a row must be whole scale blocks) or a size is 0 or 2^31 and more. */
+size_t hct_b200_int4_weight_bytes(size_t rows, size_t cols);
+/* Lays the payload of a rows x cols matrix (f16 scales, then nibbles, at any
+ * byte address) out for the products, at d_packed (128-byte aligned,
+ * hct_b200_int4_weight_bytes).  A payload shorter than rows * cols / 16 +
+ * rows * cols / 2 bytes is HCT_B200_ERR_SIZE_MISMATCH.  Stream-ordered. */
+int hct_b200_int4_weight_pack(const uint8_t *d_data, size_t data_len, size_t rows, size_t cols,
+                              void *d_packed, void *stream);
+
 /* ---- IDCT ---------------------------------------------------------------
  * haagenti_core::dct::idct_2d (crates/haagenti-core/src/dct.rs:311-337) and
  * GpuDctContext::idct_2d (crates/haagenti-cuda/src/dct_gpu.rs:1404-1412):

@@ -147,6 +147,43 @@ pub struct hct_b200_holo_info {
     pub cols: u64,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct hct_b200_linear_args {
+    pub rows: u64,
+    pub out_features: u64,
+    pub in_features: u64,
+    pub d_x: *const c_void,
+    pub ldx: u64,
+    pub d_weight: *const c_void,
+    pub ldw: u64,
+    pub weight_stride: u64,
+    pub d_bias: *const c_void,
+    pub d_gate: *const c_void,
+    pub ldgate: u64,
+    pub d_residual: *const c_void,
+    pub ldresidual: u64,
+    pub d_out: *mut c_void,
+    pub ldout: u64,
+    pub d_offsets: *const c_void,
+    pub experts: u32,
+    pub offsets_bits: i32,
+    pub x_dtype: i32,
+    pub weight_form: i32,
+    pub bias_dtype: i32,
+    pub out_dtype: i32,
+    pub activation: i32,
+    pub reserved: i32,
+}
+
+pub const HCT_B200_ACT_NONE: i32 = 0;
+pub const HCT_B200_ACT_RELU: i32 = 1;
+pub const HCT_B200_ACT_SILU: i32 = 2;
+pub const HCT_B200_ACT_GELU: i32 = 3;
+pub const HCT_B200_ACT_GELU_TANH: i32 = 4;
+pub const HCT_B200_WEIGHT_DENSE: i32 = 0;
+pub const HCT_B200_WEIGHT_INT4: i32 = 1;
+
 #[link(name = "hct_b200")]
 extern "C" {
     // ---- context
@@ -192,6 +229,15 @@ extern "C" {
     pub fn hct_b200_dequantize_int4_mp(d_data: *const u8, data_len: usize, num_elements: usize,
                                        d_out: *mut c_void, out_dtype: c_int, written: *mut usize,
                                        stream: *mut c_void) -> c_int;
+
+    // ---- products with decoded weights
+    pub fn hct_b200_linear(args: *const hct_b200_linear_args, stream: *mut c_void) -> c_int;
+    pub fn hct_b200_grouped_linear(args: *const hct_b200_linear_args, stream: *mut c_void)
+                                   -> c_int;
+    pub fn hct_b200_linear_status(stream: *mut c_void) -> c_int;
+    pub fn hct_b200_int4_weight_bytes(rows: usize, cols: usize) -> usize;
+    pub fn hct_b200_int4_weight_pack(d_data: *const u8, data_len: usize, rows: usize, cols: usize,
+                                     d_packed: *mut c_void, stream: *mut c_void) -> c_int;
 
     // ---- IDCT (dct.rs:311-337) and the spectral payload
     pub fn hct_b200_idct_2d(ctx: *mut hct_b200_ctx, d_in: *const f32, d_out: *mut c_void,
