@@ -85,47 +85,46 @@ struct LinParams {
     int bias_f32, act, odt;
 };
 
-// Rows [lo, hi) of expert e, clamped to [0, M] and to lo <= hi; without
-// offsets the one expert owns every row.
-__device__ __forceinline__ void expert_rows(const LinParams &p, uint32_t e, uint32_t &lo,
-                                            uint32_t &hi) {
-    if (!p.offsets) {
-        lo = 0;
-        hi = p.M;
-        return;
-    }
-    int64_t a, b;
-    if (p.off64) {
-        a = reinterpret_cast<const int64_t *>(p.offsets)[e];
-        b = reinterpret_cast<const int64_t *>(p.offsets)[e + 1];
-    } else {
-        a = reinterpret_cast<const int32_t *>(p.offsets)[e];
-        b = reinterpret_cast<const int32_t *>(p.offsets)[e + 1];
-    }
-    const int64_t m = (int64_t)p.M;
-    a = a < 0 ? 0 : a > m ? m : a;
-    b = b < a ? a : b > m ? m : b;
-    lo = (uint32_t)a;
-    hi = (uint32_t)b;
-}
-
-// first[e] = number of `tile`-row tiles of the experts before e, first[E] =
-// their total.  Called by one whole warp; first is shared memory.
-__device__ __forceinline__ void scan_tiles(const LinParams &p, uint32_t tile, uint32_t *first) {
+// The groups: off[e] .. off[e + 1] are the rows of expert e, first[e] is the
+// number of `tile`-row tiles of the experts before it and first[E] their total.
+// Offsets are clamped to [0, M] and to the largest before them, so that groups
+// never overlap; without offsets the one expert owns every row.  Called by one
+// whole warp; both arrays are shared memory, of E + 1 entries.
+__device__ __forceinline__ void scan_groups(const LinParams &p, uint32_t tile, uint32_t *first,
+                                            uint32_t *off) {
     const uint32_t lane = threadIdx.x & 31u;
+    uint32_t most = 0;  // largest offset so far
+    for (uint32_t i0 = 0; i0 <= p.E; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        int64_t v = 0;
+        if (i <= p.E) {
+            if (!p.offsets) v = i ? p.M : 0;
+            else if (p.off64) v = reinterpret_cast<const int64_t *>(p.offsets)[i];
+            else v = reinterpret_cast<const int32_t *>(p.offsets)[i];
+        }
+        uint32_t o = v < 0 ? 0u : v > (int64_t)p.M ? p.M : (uint32_t)v;
+        o = max(o, most);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t w = __shfl_up_sync(0xffffffffu, o, d);
+            if (lane >= (uint32_t)d) o = max(o, w);
+        }
+        if (i <= p.E) off[i] = o;
+        most = __shfl_sync(0xffffffffu, o, 31);
+    }
+    __syncwarp();
     uint32_t base = 0;
     for (uint32_t e0 = 0; e0 < p.E; e0 += 32) {
         const uint32_t e = e0 + lane;
-        uint32_t lo = 0, hi = 0;
-        if (e < p.E) expert_rows(p, e, lo, hi);
-        uint32_t c = (hi - lo + tile - 1) / tile, s = c;
+        const uint32_t c = e < p.E ? (off[e + 1] - off[e] + tile - 1) / tile : 0;
+        uint32_t sum = c;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, s, d);
-            if (lane >= (uint32_t)d) s += v;
+            const uint32_t w = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= (uint32_t)d) sum += w;
         }
-        if (e < p.E) first[e] = base + s - c;
-        base += __shfl_sync(0xffffffffu, s, 31);
+        if (e < p.E) first[e] = base + sum - c;
+        base += __shfl_sync(0xffffffffu, sum, 31);
     }
     if (lane == 0) first[p.E] = base;
     __syncwarp();
@@ -189,6 +188,8 @@ __device__ __forceinline__ void finish(const LinParams &p, uint32_t m, uint32_t 
     store_out(p.out, (uint64_t)m * p.ldo + n, p.odt, y);
 }
 
+__device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has expired
+
 // ---- plain kernel: any alignment, any stride ------------------------------------
 //
 // 32 rows x 64 features per CTA, 32-wide K steps through shared memory, f32
@@ -198,10 +199,10 @@ constexpr int SM_M = 32, SM_N = 64, SM_K = 32, SM_THREADS = 256;
 
 template <bool BF, bool INT4>
 __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParams p) {
-    __shared__ uint32_t first[MAX_EXPERTS + 1];
+    __shared__ uint32_t first[MAX_EXPERTS + 1], off[MAX_EXPERTS + 1];
     __shared__ float xs[SM_K][SM_M + 1], ws[SM_K][SM_N + 1];
     const uint32_t tid = threadIdx.x;
-    if (tid < 32) scan_tiles(p, SM_M, first);
+    if (tid < 32) scan_groups(p, SM_M, first, off);
     __syncthreads();
     const uint32_t n_tiles = (p.N + SM_N - 1) / SM_N;
     const uint64_t tiles = (uint64_t)first[p.E] * n_tiles;
@@ -209,9 +210,7 @@ __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParam
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const uint32_t mt = (uint32_t)(t / n_tiles), n0 = (uint32_t)(t % n_tiles) * SM_N;
         const uint32_t e = expert_of(first, p.E, mt);
-        uint32_t lo, hi;
-        expert_rows(p, e, lo, hi);
-        const uint32_t m0 = lo + (mt - first[e]) * SM_M;
+        const uint32_t hi = off[e + 1], m0 = off[e] + (mt - first[e]) * SM_M;
         float acc[2][4] = {};
         for (uint32_t k0 = 0; k0 < p.K; k0 += SM_K) {
             for (uint32_t i = tid; i < SM_M * SM_K; i += SM_THREADS) {
@@ -267,7 +266,635 @@ __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParam
     }
 }
 
-__device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has expired
+// ---- tensor-core kernel ---------------------------------------------------------
+//
+// A tile is 128 output features x up to BN rows of x, computed transposed:
+// the weights are the M side of the tcgen05 contraction (A, 128 rows, K-major)
+// and the rows of x its N side (B), so that one token costs an instruction of
+// width 16 instead of an almost empty 128-row tile, and INT4 weights are
+// dequantised straight into the A operand.  The instruction's N is the tile's
+// own row count rounded up to 16.
+//
+//   warp 0      TMA producer: x tiles (and dense weight tiles) into a ring of
+//               K steps of 64, packed INT4 blocks into a ring of their own
+//   warp 1      TMEM allocation; one thread issues the MMAs
+//   warps 4-7   epilogue: accumulator (TMEM lanes = features) to outputs; a
+//               warp's 32 lanes hold 32 consecutive features of a row
+//   warps 8-15  INT4 only: two groups of 128 threads dequantise every other
+//               K step, a thread per weight row, into the 128B-swizzled A tile
+//
+// With at least one tile per SM the kernel is persistent (grid = SMs) and the
+// accumulators are double-buffered, so a tile's epilogue runs under the next
+// tile's MMAs.  With fewer, the K range of a tile is split over a cluster of
+// CTAs, whose partial sums meet in distributed shared memory and are added in
+// rank order: no workspace, no atomics, the same bits every time.
+//
+// F32 outputs (PRECISE) accumulate at most SECTION K steps in TMEM and add the
+// sections in registers with rounding; INT4 weights are then two A operands,
+// the rounded weight and what the rounding left.
+//
+// Every wait is bounded; an expired one raises g_linear_status, the CTA's
+// roles leave their loops, its copies and MMAs are drained (bounded) and TMEM
+// is freed.
+constexpr int BK = 64;  // 128 bytes of a row: one swizzle row
+constexpr int A_BYTES = 128 * BK * 2;
+constexpr int MAX_STAGES = 8, MAX_RAW = 16;
+constexpr int SECTION = 4;
+constexpr int PRECISE_BN = 64;
+constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KB
+constexpr uint32_t SMEM_MIN = 120 * 1024;  // one CTA per SM: TMEM is never waited for
+constexpr uint32_t RASTER = 8;
+
+struct UmmaParams {
+    LinParams p;
+    uint32_t bn;      // rows per tile at most (a multiple of xbox)
+    uint32_t xbox;    // rows per TMA box of x (a multiple of 16)
+    uint32_t stages, raw_stages;
+    uint32_t tmem_cols, tmem_stride;
+    uint32_t split;   // CTAs per cluster, each a part of K
+};
+
+struct Ctl {
+    uint64_t xfull[MAX_STAGES], afull[MAX_STAGES], empty[MAX_STAGES];
+    uint64_t rfull[MAX_RAW], rempty[MAX_RAW];
+    uint64_t tfull[2], tempty[2], drain;
+    uint32_t tmem_base;
+    int abort, issued, raw_issued;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ uint64_t globaltimer() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait (2 s): false when the phase did not complete in time.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer();
+    for (uint32_t i = 1; i < (1u << 30); ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 0 && globaltimer() - t0 > 2000000000ull) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x,
+                                       int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x,
+                                       int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            dst),
+        "l"(src), "r"(bytes), "r"(bar)
+        : "memory");
+}
+// K-major, 128B swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                     uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// One tile: expert, its rows [m0, m0 + rows) and first feature n0.
+struct Tile {
+    uint32_t e, m0, rows, n0;
+};
+__device__ __forceinline__ Tile tile_at(const UmmaParams &u, const uint32_t *first,
+                                        const uint32_t *off, uint32_t t) {
+    const LinParams &p = u.p;
+    const uint32_t nt = (p.N + 127) / 128;
+    Tile r;
+    r.e = expert_of(first, p.E, t / nt);
+    const uint32_t lo = off[r.e], hi = off[r.e + 1], m = hi - lo, mts = (m + u.bn - 1) / u.bn;
+    // rows dealt out evenly, in whole instruction widths
+    const uint32_t per = ((m + mts - 1) / mts + 15) / 16 * 16;
+    // groups of RASTER row tiles; within one, the row tiles of a feature tile
+    // run next to each other, so that the tiles in flight share x and w in L2
+    const uint32_t q = t - first[r.e] * nt;
+    const uint32_t grp = q / (RASTER * nt), in = q - grp * RASTER * nt;
+    const uint32_t width = min(RASTER, mts - grp * RASTER);
+    const uint32_t mt = grp * RASTER + in % width;
+    r.n0 = in / width * 128;
+    r.m0 = lo + mt * per;
+    r.rows = min(per, hi - r.m0);
+    return r;
+}
+
+// Eight INT4 values times their scale as four pairs of x's type, and for
+// PRECISE what the rounding of each left.
+//
+// (word >> 4 j) & 0x000f000f are the nibbles of the pair (2 j, 2 j + 1); or'ed
+// into the mantissa of 1024 (fp16) or 128 (bf16) they are 1024 + n or 128 + n
+// exactly, and n - 8 after an exact subtraction.  fp16: one multiplication by
+// the scale, rounded once.  bf16: the f16 scale (11 bits) is hi + lo, two
+// bf16 values; (n - 8) lo has at most 6 bits, so fma(n - 8, hi, (n - 8) lo)
+// rounds the exact product once.
+template <bool BF>
+struct Scale;
+template <>
+struct Scale<false> {
+    __half2 s;
+    bool finite;
+    __device__ __forceinline__ explicit Scale(uint16_t b) {
+        s = __half2half2(__ushort_as_half(b));
+        finite = (b & 0x7c00u) != 0x7c00u;
+    }
+};
+template <>
+struct Scale<true> {
+    __nv_bfloat162 hi, lo;
+    bool finite;
+    __device__ __forceinline__ explicit Scale(uint16_t b) {
+        const float f = h2f(b);
+        const __nv_bfloat16 h = __float2bfloat16_rn(f);
+        finite = (b & 0x7c00u) != 0x7c00u;
+        hi = __bfloat162bfloat162(h);
+        lo = __bfloat162bfloat162(__float2bfloat16_rn(finite ? f - __bfloat162float(h) : 0.0f));
+    }
+};
+template <class T>
+__device__ __forceinline__ uint32_t bits_of(T v) {
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+template <bool PRECISE>
+__device__ __forceinline__ void dequant8(uint32_t w, const Scale<false> &s, uint32_t (&v)[4],
+                                         uint32_t (&l)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t b = ((w >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+        const __half2 n = __hsub2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(1032.0f));
+        const __half2 h = __hmul2(n, s.s);
+        v[j] = bits_of(h);
+        if (PRECISE) l[j] = s.finite ? bits_of(__hfma2(n, s.s, __hneg2(h))) : 0u;
+    }
+}
+template <bool PRECISE>
+__device__ __forceinline__ void dequant8(uint32_t w, const Scale<true> &s, uint32_t (&v)[4],
+                                         uint32_t (&l)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t b = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 n =
+            __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&b), __float2bfloat162_rn(136.0f));
+        const __nv_bfloat162 c = __hmul2(n, s.lo);
+        const __nv_bfloat162 h = __hfma2(n, s.hi, c);
+        v[j] = bits_of(h);
+        if (PRECISE) l[j] = s.finite ? bits_of(__hadd2(__hfma2(n, s.hi, __hneg2(h)), c)) : 0u;
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void activate16(float (&z)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) z[j] = activate(z[j], ACT);
+}
+
+// Sixteen rows m .. m + 15 (count of them live) of feature n: sums to outputs.
+template <bool BF, int ODT>
+__device__ __forceinline__ void finish16(const LinParams &p, float (&z)[16], float bias, uint32_t m,
+                                         uint32_t count, uint32_t n) {
+    float g[16], r[16];
+    if (p.gate) {
+        const uint16_t *q = reinterpret_cast<const uint16_t *>(p.gate) + (uint64_t)m * p.ldgate + n;
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            g[j] = j < (int)count ? from16<BF>(q[(uint64_t)j * p.ldgate]) : 0.0f;
+    }
+    if (p.res) {
+        const uint64_t at = (uint64_t)m * p.ldres + n;
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            r[j] = j < (int)count ? load_out_type(p.res, at + (uint64_t)j * p.ldres, ODT) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) z[j] += bias;
+    switch (p.act) {
+        case HCT_B200_ACT_RELU: activate16<HCT_B200_ACT_RELU>(z); break;
+        case HCT_B200_ACT_SILU: activate16<HCT_B200_ACT_SILU>(z); break;
+        case HCT_B200_ACT_GELU: activate16<HCT_B200_ACT_GELU>(z); break;
+        case HCT_B200_ACT_GELU_TANH: activate16<HCT_B200_ACT_GELU_TANH>(z); break;
+        default: break;
+    }
+    if (p.gate) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) z[j] *= g[j];
+    }
+    if (p.res) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) z[j] += r[j];
+    }
+    const uint64_t at = (uint64_t)m * p.ldo + n;
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+        if (j < (int)count) store_out(p.out, at + (uint64_t)j * p.ldo, ODT, z[j]);
+}
+
+constexpr int umma_threads(bool int4) { return int4 ? 512 : 256; }
+
+template <bool INT4, bool BF, bool PRECISE>
+__global__ void __launch_bounds__(umma_threads(INT4), 1)
+    linear_umma_kernel(const __grid_constant__ CUtensorMap tmX,
+                       const __grid_constant__ CUtensorMap tmW, const __grid_constant__ UmmaParams u) {
+    constexpr uint32_t A_PARTS = INT4 && PRECISE ? 2 : 1;
+    constexpr int GROUPS = 2;  // of dequantising warps
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const LinParams &p = u.p;
+    const uint32_t stages = u.stages, stage_bytes = A_PARTS * A_BYTES + u.bn * 128;
+    uint8_t *raw = smem + (size_t)stages * stage_bytes;
+    Ctl *ctl = reinterpret_cast<Ctl *>(raw + (size_t)u.raw_stages * PK_BYTES);
+    uint32_t *first = reinterpret_cast<uint32_t *>(ctl + 1), *off = first + p.E + 1;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < stages; s++) {
+            mbar_init(smem_u32(&ctl->xfull[s]), 1);
+            mbar_init(smem_u32(&ctl->afull[s]), 4);
+            mbar_init(smem_u32(&ctl->empty[s]), 1);
+        }
+        for (uint32_t s = 0; s < u.raw_stages; s++) {
+            mbar_init(smem_u32(&ctl->rfull[s]), 1);
+            mbar_init(smem_u32(&ctl->rempty[s]), 4);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(smem_u32(&ctl->tfull[b]), 1);
+            mbar_init(smem_u32(&ctl->tempty[b]), 4);
+        }
+        mbar_init(smem_u32(&ctl->drain), 1);
+        ctl->abort = 0;
+        ctl->issued = 0;
+        ctl->raw_issued = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&ctl->tmem_base)),
+                     "r"(u.tmem_cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    if (warp == 2) scan_groups(p, u.bn, first, off);
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = ctl->tmem_base;
+    const auto aborted = [&] { return *(volatile int *)&ctl->abort != 0; };
+    const auto give_up = [&] {
+        atomicExch(&g_linear_status, HCT_B200_ERR_TIMEOUT);
+        atomicExch(&ctl->abort, 1);
+    };
+
+    const uint32_t nt = (p.N + 127) / 128;
+    const uint32_t tiles = first[p.E] * nt;
+    const uint32_t rank = blockIdx.x % u.split;  // clusters are consecutive CTAs
+    const uint32_t t0 = blockIdx.x / u.split, step = gridDim.x / u.split;
+    const uint32_t kbs = (p.K + BK - 1) / BK;
+    const uint32_t kb0 = (uint32_t)((uint64_t)kbs * rank / u.split);
+    const uint32_t kb1 = (uint32_t)((uint64_t)kbs * (rank + 1) / u.split);
+    const uint32_t sect = PRECISE ? SECTION : kb1 - kb0;  // K steps per accumulation
+
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+            if (!INT4)
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW))
+                             : "memory");
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t t = t0; ok && t < tiles; t += step) {
+                const Tile c = tile_at(u, first, off, t);
+                const uint32_t boxes = (c.rows + u.xbox - 1) / u.xbox;
+                for (uint32_t kb = kb0; kb < kb1; kb++, it++) {
+                    const uint32_t s = it % stages, ph = (it / stages) & 1u;
+                    if (aborted() || !mbar_wait(smem_u32(&ctl->empty[s]), ph ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sa = smem_u32(smem + (size_t)s * stage_bytes);
+                    const uint32_t sb = sa + A_PARTS * A_BYTES, fb = smem_u32(&ctl->xfull[s]);
+                    mbar_expect_tx(fb, boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES));
+                    if (!INT4) tma_3d(sa, &tmW, fb, (int)(kb * BK), (int)c.n0, (int)c.e);
+                    for (uint32_t b = 0; b < boxes; b++)
+                        tma_2d(sb + b * u.xbox * 128, &tmX, fb, (int)(kb * BK),
+                               (int)(c.m0 + b * u.xbox));
+                    *(volatile int *)&ctl->issued = (int)(it + 1);
+                }
+            }
+            if (!ok) give_up();
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // D = F32, A = B = x's type, both K-major, M = 128; N follows the tile
+            const uint32_t idesc0 = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);
+            uint32_t it = 0, use = 0;
+            bool ok = true;
+            for (uint32_t t = t0; ok && t < tiles; t += step) {
+                const Tile c = tile_at(u, first, off, t);
+                const uint32_t idesc = idesc0 | ((c.rows + 15) / 16 * 2) << 17;
+                for (uint32_t kb = kb0; ok && kb < kb1; use++) {
+                    const uint32_t end = min(kb + sect, kb1), buf = use & 1u;
+                    if (!mbar_wait(smem_u32(&ctl->tempty[buf]), ((use >> 1) & 1u) ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d = tmem + buf * u.tmem_stride;
+                    for (uint32_t from = kb; kb < end; kb++, it++) {
+                        const uint32_t s = it % stages, ph = (it / stages) & 1u;
+                        if (aborted() || !mbar_wait(smem_u32(&ctl->xfull[s]), ph) ||
+                            (INT4 && !mbar_wait(smem_u32(&ctl->afull[s]), ph))) {
+                            ok = false;
+                            break;
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t sa = smem_u32(smem + (size_t)s * stage_bytes);
+                        const uint64_t db = umma_desc(sa + A_PARTS * A_BYTES);
+#pragma unroll
+                        for (uint32_t a = 0; a < A_PARTS; a++) {
+                            const uint64_t da = umma_desc(sa + a * A_BYTES);
+#pragma unroll
+                            for (uint32_t k = 0; k < BK / 16; k++)
+                                umma(d, da + 2 * k, db + 2 * k, idesc, kb != from || a || k);
+                        }
+                        umma_commit(smem_u32(&ctl->empty[s]));
+                    }
+                    if (ok) umma_commit(smem_u32(&ctl->tfull[buf]));
+                }
+            }
+            if (!ok) give_up();
+            umma_commit(smem_u32(&ctl->drain));  // completes once every MMA above has
+        }
+    } else if (INT4 && warp == 3) {
+        if (lane == 0) {
+            const uint64_t per_expert = (uint64_t)nt * kbs;
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t t = t0; ok && t < tiles; t += step) {
+                const Tile c = tile_at(u, first, off, t);
+                const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
+                                     (c.e * per_expert + (uint64_t)(c.n0 / 128) * kbs + kb0) * PK_BYTES;
+                for (uint32_t kb = kb0; kb < kb1; kb++, it++, src += PK_BYTES) {
+                    const uint32_t r = it % u.raw_stages, ph = (it / u.raw_stages) & 1u;
+                    if (aborted() || !mbar_wait(smem_u32(&ctl->rempty[r]), ph ^ 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = smem_u32(&ctl->rfull[r]);
+                    mbar_expect_tx(fb, PK_BYTES);
+                    bulk_load(smem_u32(raw + (size_t)r * PK_BYTES), src, PK_BYTES, fb);
+                    *(volatile int *)&ctl->raw_issued = (int)(it + 1);
+                }
+            }
+            if (!ok) give_up();
+        }
+    } else if (INT4 && warp >= 8) {
+        const uint32_t group = (warp - 8) >> 2, row = threadIdx.x & 127u;
+        uint32_t it = 0;
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += step) {
+            for (uint32_t kb = kb0; kb < kb1; kb++, it++) {
+                if (it % GROUPS != group) continue;
+                const uint32_t r = it % u.raw_stages, s = it % stages;
+                if (aborted() || !mbar_wait(smem_u32(&ctl->rfull[r]), (it / u.raw_stages) & 1u)) {
+                    ok = false;
+                    break;
+                }
+                const uint8_t *src = raw + (size_t)r * PK_BYTES;
+                uint4 q[2];
+                uint16_t sc[2];
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    q[g] = *reinterpret_cast<const uint4 *>(src + (g * 128 + row) * 16);
+                    sc[g] = *reinterpret_cast<const uint16_t *>(src + PK_NIB + (g * 128 + row) * 2);
+                }
+                if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / stages) & 1u) ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *a = smem + (size_t)s * stage_bytes + row * 128;
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const Scale<BF> scale(sc[g]);
+                    const uint32_t w[4] = {q[g].x, q[g].y, q[g].z, q[g].w};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t v[4], l[4];
+                        dequant8<PRECISE>(w[c], scale, v, l);
+                        uint8_t *o = a + (((g * 4 + c) ^ (row & 7u)) << 4);
+                        *reinterpret_cast<uint4 *>(o) = make_uint4(v[0], v[1], v[2], v[3]);
+                        if (PRECISE)
+                            *reinterpret_cast<uint4 *>(o + A_BYTES) = make_uint4(l[0], l[1], l[2], l[3]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&ctl->afull[s]));
+                    mbar_arrive(smem_u32(&ctl->rempty[r]));
+                }
+            }
+        }
+        if (!ok) give_up();
+    } else if (warp >= 4 && warp < 8) {
+        const uint32_t q = warp & 3u, row = q * 32 + lane;
+        float *part = reinterpret_cast<float *>(smem);  // split: [rows of x][128 features]
+        uint32_t use = 0;
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += step) {
+            const Tile c = tile_at(u, first, off, t);
+            const uint32_t n = c.n0 + row;
+            const bool live = n < p.N;
+            const float bias = live && u.split == 1 ? bias_of<BF>(p, c.e, n) : 0.0f;
+            if (!PRECISE) {
+                const uint32_t buf = use & 1u;
+                if (!mbar_wait(smem_u32(&ctl->tfull[buf]), (use >> 1) & 1u) || aborted()) {
+                    ok = false;
+                    break;
+                }
+                use++;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t ta = tmem + buf * u.tmem_stride + ((q * 32) << 16);
+                for (uint32_t j0 = 0; j0 < c.rows; j0 += 16) {
+                    uint32_t v[16];
+                    float z[16];
+                    __syncwarp();
+                    tmem_ld16(ta + j0, v);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) z[j] = __uint_as_float(v[j]);
+                    if (u.split > 1) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + row] = z[j];
+                    } else if (live) {
+                        const uint32_t count = min(16u, c.rows - j0);
+                        if (p.odt == HCT_B200_F16)
+                            finish16<BF, HCT_B200_F16>(p, z, bias, c.m0 + j0, count, n);
+                        else
+                            finish16<BF, HCT_B200_BF16>(p, z, bias, c.m0 + j0, count, n);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[buf]));
+            } else {
+                float z[PRECISE_BN / 16][16];
+#pragma unroll
+                for (int i = 0; i < PRECISE_BN / 16; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) z[i][j] = 0.0f;
+                for (uint32_t kb = kb0; kb < kb1; kb += sect, use++) {
+                    const uint32_t buf = use & 1u;
+                    if (!mbar_wait(smem_u32(&ctl->tfull[buf]), (use >> 1) & 1u) || aborted()) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t ta = tmem + buf * u.tmem_stride + ((q * 32) << 16);
+#pragma unroll
+                    for (int i = 0; i < PRECISE_BN / 16; i++) {
+                        if (i * 16 >= (int)c.rows) continue;
+                        uint32_t v[16];
+                        __syncwarp();
+                        tmem_ld16(ta + i * 16, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) z[i][j] += __uint_as_float(v[j]);
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[buf]));
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < PRECISE_BN / 16; i++) {
+                    if (i * 16 >= (int)c.rows) continue;
+                    if (u.split > 1) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) part[(i * 16 + j) * 128 + row] = z[i][j];
+                    } else if (live) {
+                        finish16<BF, HCT_B200_F32>(p, z[i], bias, c.m0 + i * 16,
+                                                   min(16u, c.rows - i * 16), n);
+                    }
+                }
+            }
+        }
+        if (!ok) give_up();
+    }
+
+    if (u.split > 1) {
+        // one tile per cluster: each CTA finishes its share of the tile's rows,
+        // adding the CTAs' parts in rank order.  Both barriers are reached by
+        // every thread of every CTA on every path.
+        __syncwarp();
+        cluster_barrier();
+        if (t0 < tiles && !aborted()) {
+            const Tile c = tile_at(u, first, off, t0);
+            const uint32_t j0 = c.rows * rank / u.split, j1 = c.rows * (rank + 1) / u.split;
+            const uint32_t f = threadIdx.x & 127u, n = c.n0 + f;
+            const uint32_t base = smem_u32(smem);
+            if (n < p.N) {
+                const float bias = bias_of<BF>(p, c.e, n);
+                for (uint32_t j = j0 + threadIdx.x / 128; j < j1; j += blockDim.x / 128) {
+                    float z = 0.0f;
+                    for (uint32_t r = 0; r < u.split; r++) z += ld_cluster(base + (j * 128 + f) * 4, r);
+                    finish<BF>(p, c.m0 + j, n, z + bias);
+                }
+            }
+        }
+        cluster_barrier();
+    }
+
+    // ---- teardown: nothing of this CTA may be in flight when it ends --------------
+    __syncthreads();
+    if (threadIdx.x == 0 && aborted()) {
+        // the latest load into each slot (its phase completes only with the copy)
+        const int issued = *(volatile int *)&ctl->issued, got = *(volatile int *)&ctl->raw_issued;
+        for (int it = max(0, issued - (int)stages); it < issued; it++)
+            if (!mbar_wait(smem_u32(&ctl->xfull[it % stages]), (uint32_t)(it / stages) & 1u)) give_up();
+        for (int it = max(0, got - (int)u.raw_stages); it < got; it++)
+            if (!mbar_wait(smem_u32(&ctl->rfull[it % u.raw_stages]),
+                           (uint32_t)(it / u.raw_stages) & 1u))
+                give_up();
+    }
+    if (threadIdx.x == 32 && !mbar_wait(smem_u32(&ctl->drain), 0)) give_up();
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(u.tmem_cols)
+                     : "memory");
+    }
+}
 
 // ---- host side --------------------------------------------------------------------
 
@@ -373,6 +1000,139 @@ int check(const hct_b200_linear_args *a, bool grouped, bool *nothing) {
     return HCT_B200_OK;
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                   const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                   const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void *q = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) !=
+                cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            q = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(q);
+    }();
+    return fn;
+}
+
+// rows of K 16-bit values, `ld` apart, in `batch` matrices `bstride` apart:
+// boxes of 64 values x box_rows rows of one matrix.  A 2-D map when batch is 0.
+bool operand_map(CUtensorMap *map, bool bf, const void *base, uint64_t K, uint64_t rows, uint64_t ld,
+                 uint64_t batch, uint64_t bstride, uint32_t box_rows) {
+    const cuuint64_t dims[3] = {K, rows, batch};
+    const cuuint64_t strides[2] = {ld * 2, bstride * 2};
+    const cuuint32_t box[3] = {BK, box_rows, 1}, one[3] = {1, 1, 1};
+    return encode_fn() &&
+           encode_fn()(map,
+                       bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                       batch ? 3 : 2, const_cast<void *>(base), dims, strides, box, one,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows that TMA can fetch: 16-byte aligned starts, no two rows overlapping.
+bool tma_rows(const void *base, uint64_t rows, uint64_t ld, uint64_t K) {
+    return (uintptr_t)base % 16 == 0 && (rows == 1 || (ld % 8 == 0 && ld >= K));
+}
+
+inline uint32_t round_to(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
+
+template <bool INT4, bool BF, bool PRECISE>
+cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const UmmaParams &u,
+                        uint32_t grid, uint32_t smem, cudaStream_t s) {
+    const auto kernel = linear_umma_kernel<INT4, BF, PRECISE>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)SMEM_LIMIT);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(umma_threads(INT4));
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = u.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    c.attrs = attr;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, tx, tw, u);
+}
+
+// Tile height, split and ring depths of a call on the tensor-core kernel.
+cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaStream_t s) {
+    const bool precise = p.odt == HCT_B200_F32;
+    const uint32_t sms = (uint32_t)sm_count(), cap = precise ? PRECISE_BN : 256;
+    const uint32_t nt = (p.N + 127) / 128, kbs = (p.K + BK - 1) / BK;
+    UmmaParams u{};
+    u.p = p;
+    uint64_t row_tiles;  // at most
+    if (!grouped) {
+        if (p.M <= cap) {
+            u.bn = round_to(p.M, 16);
+        } else {
+            // the height whose waves of tiles take the least time: waves x (rows +
+            // what a tile costs beside its rows)
+            uint64_t best = ~0ull;
+            for (uint32_t bn = cap; bn >= cap / 2; bn -= 16) {
+                const uint64_t mts = (p.M + bn - 1) / bn;
+                const uint32_t per = round_to((uint32_t)((p.M + mts - 1) / mts), 16);
+                const uint64_t cost = (mts * nt + sms - 1) / sms * (per + 16);
+                if (cost < best) {
+                    best = cost;
+                    u.bn = bn;
+                }
+            }
+        }
+        u.xbox = u.bn;
+        row_tiles = (p.M + u.bn - 1) / u.bn;
+    } else {
+        const uint32_t active = std::min(p.E, p.M);
+        u.bn = std::min(cap, p.M / active <= 64 ? 128u : 256u);
+        u.xbox = 32;
+        row_tiles = p.M / u.bn + active;
+    }
+    const uint64_t tiles = row_tiles * nt;
+    if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
+    // fewer tiles than half the SMs: the K range is split over a cluster
+    u.split = 1;
+    if (tiles * 2 <= sms) u.split = std::min<uint32_t>({8u, (uint32_t)(sms / tiles), kbs});
+    const uint32_t grid = u.split > 1 ? (uint32_t)tiles * u.split
+                                      : (uint32_t)std::min<uint64_t>(tiles, sms);
+    u.tmem_stride = round_to(u.bn, 32);
+    u.tmem_cols = 64;
+    while (u.tmem_cols < 2 * u.tmem_stride) u.tmem_cols *= 2;
+    const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn * 128;
+    u.raw_stages = int4 ? 10 : 0;
+    const uint32_t fixed = 1024 + u.raw_stages * PK_BYTES + (uint32_t)sizeof(Ctl) + (p.E + 1) * 8;
+    u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
+    const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
+
+    alignas(64) CUtensorMap tx, tw;
+    if (!operand_map(&tx, bf, p.x, p.K, p.M, p.M == 1 ? round_to(p.K, 8) : p.ldx, 0, 0, u.xbox))
+        return cudaErrorInvalidValue;
+    if (int4) {
+        tw = tx;
+    } else {
+        const uint64_t ld = p.N == 1 ? round_to(p.K, 8) : p.ldw;
+        if (!operand_map(&tw, bf, p.w, p.K, p.N, ld, p.E, p.E == 1 ? ld * p.N : p.w_stride, 128))
+            return cudaErrorInvalidValue;
+    }
+    if (int4) {
+        if (bf) return precise ? launch_umma<true, true, true>(tx, tw, u, grid, smem, s)
+                               : launch_umma<true, true, false>(tx, tw, u, grid, smem, s);
+        return precise ? launch_umma<true, false, true>(tx, tw, u, grid, smem, s)
+                       : launch_umma<true, false, false>(tx, tw, u, grid, smem, s);
+    }
+    if (bf) return precise ? launch_umma<false, true, true>(tx, tw, u, grid, smem, s)
+                           : launch_umma<false, true, false>(tx, tw, u, grid, smem, s);
+    return precise ? launch_umma<false, false, true>(tx, tw, u, grid, smem, s)
+                   : launch_umma<false, false, false>(tx, tw, u, grid, smem, s);
+}
+
 int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     bool nothing = false;
     const int rc = check(a, grouped, &nothing);
@@ -400,6 +1160,10 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     p.act = a->activation;
     p.odt = a->out_dtype;
     const bool bf = a->x_dtype == HCT_B200_BF16, int4 = a->weight_form == HCT_B200_WEIGHT_INT4;
+    // the tensor cores take rows that TMA can fetch (and strides that its maps can hold)
+    const bool w_ok = int4 || (tma_rows(p.w, p.N, p.ldw, p.K) &&
+                               (p.E == 1 || (p.w_stride % 8 == 0 && p.w_stride && p.w_stride < 1ull << 38)));
+    if (p.K && w_ok && tma_rows(p.x, p.M, p.ldx, p.K)) return code_of(run_umma(p, grouped, int4, bf, s));
     // at most this many row tiles: one partial tile per expert beside the whole ones
     const uint64_t mt = p.M / SM_M + std::min<uint64_t>(p.E, p.M);
     const uint64_t tiles = mt * ((p.N + SM_N - 1) / SM_N);

@@ -245,9 +245,10 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * grouped_linear: rows [offsets[e], offsets[e+1]) are multiplied by expert e's
  * matrix (and bias).  offsets is read on the device, with no host
  * synchronisation: experts + 1 ascending values.  Rows before offsets[0] and
- * from offsets[experts] on are neither read nor written.  Values outside
- * [0, rows] are clamped to it and a pair that descends is an empty group, so
- * that wrong offsets give wrong rows and no access out of range.
+ * from offsets[experts] on take no part and are not written.  A value outside
+ * [0, rows] is clamped to it and one below its predecessors counts as the
+ * largest of them, so that wrong offsets give wrong rows and no access out of
+ * range.
  *
  * Types: x F16 or BF16, gate of x's type; bias of x's type or F32; residual
  * of out's type; out F16, BF16 or F32.  Sums are held in f32 and the result is
@@ -256,7 +257,8 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * do not show; F32 outputs are therefore summed in sections of 256 that are
  * added with rounding.  INT4 weights are (nibble - 8) * scale: rounded to
  * x's type as hct_b200_dequantize_int4 rounds them for 16-bit outputs, and
- * held exactly (as the sum of two values of x's type) for F32 outputs.
+ * held exactly (as the sum of two values of x's type) for F32 outputs; in F16
+ * a weight beyond 65504 is infinite.
  *
  * Strides are in elements.  Rows of x and w that start on 16-byte boundaries
  * take the tensor-core path; others are handled by a slower kernel.  out may

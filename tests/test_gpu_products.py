@@ -244,7 +244,7 @@ def test_grouped_equals_linear_per_expert(hb, dev, form):
 
 @pytest.mark.parametrize("form", ["int4", "dense"])
 def test_wrong_offsets_stay_in_range(hb, dev, form):
-    """Values outside [0, rows] are clamped, descending pairs are empty groups."""
+    """Values outside [0, rows] are clamped, descending ones count as the largest before."""
     n, k, m, e = 96, 128, 50, 4
     d = make(dev, 9, m, n, k, e, form, "f16", "f16", False, False, False)
     w = hb.Int4Weight(d["w"], n, k) if form == "int4" else torch.stack(d["w"])
@@ -255,17 +255,13 @@ def test_wrong_offsets_stay_in_range(hb, dev, form):
     assert (buf[:20] == 7).all() and (buf[20 + m:] == 7).all()
     for i, q in ((0, slice(0, 4)), (2, slice(10, 30)), (3, slice(30, 50))):
         wi = weight64(d["w"][i], n, k) if form == "int4" else d["w"][i]
-        # expert 0 owns [0, 10); rows 4..9 belong to experts 0 and 2 both
+        # the groups are [0, 10), none, [10, 30) and [30, 50)
         want, tol = define(d["x"][q], wi, None, 0, None, None, torch.float16, form == "int4")
         check(y[q], want, tol, i)
     off = torch.tensor([1 << 40, -(1 << 40), 1 << 62, -1, 7], dtype=torch.int64, device=dev)
     y.fill_(7)
     hb.grouped_linear(d["x"], w, off, out=y)
-    # pairs: empty, [0, 50) once clamped, empty, [0, 7): experts 1 and 3 both own rows 0..6
-    assert (buf[:20] == 7).all() and (buf[20 + m:] == 7).all()
-    wi = weight64(d["w"][1], n, k) if form == "int4" else d["w"][1]
-    want, tol = define(d["x"][7:], wi, None, 0, None, None, torch.float16, form == "int4")
-    check(y[7:], want, tol)
+    assert (buf == 7).all()  # every group begins and ends at row 50
 
 
 @pytest.mark.parametrize("form,out", [("int4", "bf16"), ("int4", "f32"), ("dense", "bf16"),
@@ -303,10 +299,9 @@ def test_int4_scales_at_the_edges(hb, dev):
                 got = hb.linear(x, hb.Int4Weight(data, n, k), out_dtype=TAG[out])
                 fine = [i for i in range(n) if i not in (4, 5)]
                 want, tol = define(x, w[fine], None, 0, None, None, DT[out], True)
-                if dt == "f16" and out == "f16":
-                    # a subnormal weight is rounded to half a step of 2^-24, and 8 x 65504 leaves
-                    # the type: row 3 is infinite there
-                    tol = tol + x.double().abs().sum(1, keepdim=True) * 2.0 ** -25
+                if dt == "f16":
+                    # 8 x 65504 leaves the type: row 3 is infinite in fp16.  A subnormal weight is a
+                    # multiple of 2^-24, as its scale is, so that nothing more is rounded
                     inf = fine.index(3)
                     assert not got[:, 3].isfinite().all()
                     tol[:, inf], want[:, inf] = float("inf"), 0
