@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -83,6 +84,7 @@ struct LinParams {
     uint32_t M, N, K, E;
     int off64;  // offsets are int64 (else int32)
     int bias_f32, act, odt;
+    int vec_gate, vec_res, vec_out;  // rows start on 16-byte boundaries
 };
 
 // The groups: off[e] .. off[e + 1] are the rows of expert e, first[e] is the
@@ -151,10 +153,11 @@ __device__ __forceinline__ float from16(uint16_t v) {
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case HCT_B200_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        case HCT_B200_ACT_SILU: return z / (1.0f + expf(-z));
+        // __expf and __fdividef: a few 2^-23 of the value, as the rest of the f32 epilogue
+        case HCT_B200_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
         case HCT_B200_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case HCT_B200_ACT_GELU_TANH:
-            return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+        case HCT_B200_ACT_GELU_TANH:  // (1 + tanh(t)) / 2 = 1 / (1 + e^-2t)
+            return __fdividef(z, 1.0f + __expf(-1.59576912160573071f * (z + 0.044715f * z * z * z)));
         default: return z;
     }
 }
@@ -278,9 +281,11 @@ __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParam
 //   warp 0      TMA producer: x tiles (and dense weight tiles) into a ring of
 //               K steps of 64, packed INT4 blocks into a ring of their own
 //   warp 1      TMEM allocation; one thread issues the MMAs
-//   warps 4-7   epilogue: accumulator (TMEM lanes = features) to outputs; a
-//               warp's 32 lanes hold 32 consecutive features of a row
-//   warps 8-15  INT4 only: two groups of 128 threads dequantise every other
+//   warps 4-11  epilogue, two sets of four warps that take every other 16 rows:
+//               accumulators (TMEM lanes = features) through shared memory into
+//               runs of 8 features, so that outputs, gate and residual move in
+//               16-byte pieces of a row
+//   warps 12-23 INT4 only: three groups of 128 threads dequantise every third
 //               K step, a thread per weight row, into the 128B-swizzled A tile
 //
 // With at least one tile per SM the kernel is persistent (grid = SMs) and the
@@ -300,10 +305,10 @@ constexpr int BK = 64;  // 128 bytes of a row: one swizzle row
 constexpr int A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8, MAX_RAW = 16;
 constexpr int SECTION = 4;
-constexpr int PRECISE_BN = 64;
 constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KB
 constexpr uint32_t SMEM_MIN = 120 * 1024;  // one CTA per SM: TMEM is never waited for
 constexpr uint32_t RASTER = 8;
+constexpr uint32_t EPI_BYTES = 2 * 16 * 128 * 4;  // staging of the two epilogue sets
 
 struct UmmaParams {
     LinParams p;
@@ -351,16 +356,33 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait (2 s): false when the phase did not complete in time.
+// Bounded wait (2 s): false when the phase did not complete in time.  The
+// clock is read only once the wait has become a long one.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
+    uint64_t t0 = 0;
     for (uint32_t i = 1; i < (1u << 30); ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255u) == 0 && globaltimer() - t0 > 2000000000ull) return false;
+        if ((i & 255u) == 0) {
+            const uint64_t t = globaltimer();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > 2000000000ull) return false;
+        }
     }
     return false;
 }
+
+// A position in a ring of slots: the slot and the parity of its current pass.
+struct Ring {
+    uint32_t slot, pass, size;
+    __device__ __forceinline__ explicit Ring(uint32_t n, uint32_t at = 0) : slot(at), pass(0), size(n) {}
+    __device__ __forceinline__ void step(uint32_t by = 1) {  // by <= size
+        slot += by;
+        if (slot >= size) {
+            slot -= size;
+            pass ^= 1u;
+        }
+    }
+};
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x,
                                        int y) {
     asm volatile(
@@ -418,11 +440,14 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t rank) {
+__device__ __forceinline__ float4 ld_cluster(uint32_t saddr, uint32_t rank) {
     uint32_t a;
-    float v;
+    float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
     return v;
 }
 
@@ -456,7 +481,8 @@ __device__ __forceinline__ Tile tile_at(const UmmaParams &u, const uint32_t *fir
 //
 // (word >> 4 j) & 0x000f000f are the nibbles of the pair (2 j, 2 j + 1); or'ed
 // into the mantissa of 1024 (fp16) or 128 (bf16) they are 1024 + n or 128 + n
-// exactly, and n - 8 after an exact subtraction.  fp16: one multiplication by
+// exactly, and n - 8 after an exact subtraction (fp16 has room for 1024 + 16 n
+// too, which saves the shift of every other pair).  fp16: one multiplication by
 // the scale, rounded once.  bf16: the f16 scale (11 bits) is hi + lo, two
 // bf16 values; (n - 8) lo has at most 6 bits, so fma(n - 8, hi, (n - 8) lo)
 // rounds the exact product once.
@@ -492,8 +518,12 @@ __device__ __forceinline__ void dequant8(uint32_t w, const Scale<false> &s, uint
                                          uint32_t (&l)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        uint32_t b = ((w >> (4 * j)) & 0x000f000fu) | 0x64006400u;
-        const __half2 n = __hsub2(*reinterpret_cast<__half2 *>(&b), __float2half2_rn(1032.0f));
+        // odd pairs stay where they are: 1024 + 16 n, whose sixteenth less 72 is n - 8
+        uint32_t b = (j & 1 ? (w >> (8 * (j / 2))) & 0x00f000f0u : (w >> (8 * (j / 2))) & 0x000f000fu) |
+                     0x64006400u;
+        const __half2 m = *reinterpret_cast<__half2 *>(&b);
+        const __half2 n = j & 1 ? __hfma2(m, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
+                                : __hsub2(m, __float2half2_rn(1032.0f));
         const __half2 h = __hmul2(n, s.s);
         v[j] = bits_of(h);
         if (PRECISE) l[j] = s.finite ? bits_of(__hfma2(n, s.s, __hneg2(h))) : 0u;
@@ -514,66 +544,177 @@ __device__ __forceinline__ void dequant8(uint32_t w, const Scale<true> &s, uint3
     }
 }
 
-template <int ACT>
-__device__ __forceinline__ void activate16(float (&z)[16]) {
+template <int ACT, int W>
+__device__ __forceinline__ void activate_all(float (&z)[W]) {
 #pragma unroll
-    for (int j = 0; j < 16; j++) z[j] = activate(z[j], ACT);
+    for (int j = 0; j < W; j++) z[j] = activate(z[j], ACT);
 }
 
-// Sixteen rows m .. m + 15 (count of them live) of feature n: sums to outputs.
-template <bool BF, int ODT>
-__device__ __forceinline__ void finish16(const LinParams &p, float (&z)[16], float bias, uint32_t m,
-                                         uint32_t count, uint32_t n) {
-    float g[16], r[16];
+// The operands of 8 consecutive features n .. n + 7 of row m: gate in g, the
+// residual in r (8 16-bit values in r[0..3], or 8 floats).  Whole 16-byte
+// pieces where the row allows them, else element by element.
+struct Operands {
+    uint32_t g[4], r[8];
+};
+template <int ODT>
+__device__ __forceinline__ void load_operands(const LinParams &p, uint32_t m, uint32_t n,
+                                              Operands &o) {
+    const bool whole = n + 8 <= p.N;
     if (p.gate) {
         const uint16_t *q = reinterpret_cast<const uint16_t *>(p.gate) + (uint64_t)m * p.ldgate + n;
+        if (whole && p.vec_gate) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(q);
+            o.g[0] = v.x, o.g[1] = v.y, o.g[2] = v.z, o.g[3] = v.w;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-            g[j] = j < (int)count ? from16<BF>(q[(uint64_t)j * p.ldgate]) : 0.0f;
+            for (int j = 0; j < 4; j++)
+                o.g[j] = (n + 2 * j < p.N ? q[2 * j] : 0u) |
+                         (n + 2 * j + 1 < p.N ? (uint32_t)q[2 * j + 1] << 16 : 0u);
+        }
     }
     if (p.res) {
         const uint64_t at = (uint64_t)m * p.ldres + n;
+        if (ODT == HCT_B200_F32) {
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(p.res) + at;
+            if (whole && p.vec_res) {
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-            r[j] = j < (int)count ? load_out_type(p.res, at + (uint64_t)j * p.ldres, ODT) : 0.0f;
+                for (int h = 0; h < 2; h++) {
+                    const uint4 v = reinterpret_cast<const uint4 *>(q)[h];
+                    o.r[4 * h] = v.x, o.r[4 * h + 1] = v.y, o.r[4 * h + 2] = v.z, o.r[4 * h + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) o.r[j] = n + j < p.N ? q[j] : 0u;
+            }
+        } else {
+            const uint16_t *q = reinterpret_cast<const uint16_t *>(p.res) + at;
+            if (whole && p.vec_res) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(q);
+                o.r[0] = v.x, o.r[1] = v.y, o.r[2] = v.z, o.r[3] = v.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o.r[j] = (n + 2 * j < p.N ? q[2 * j] : 0u) |
+                             (n + 2 * j + 1 < p.N ? (uint32_t)q[2 * j + 1] << 16 : 0u);
+            }
+        }
     }
-#pragma unroll
-    for (int j = 0; j < 16; j++) z[j] += bias;
+}
+
+template <int ODT>
+__device__ __forceinline__ uint32_t to16(float v) {
+    return ODT == HCT_B200_F16 ? (uint32_t)__half_as_ushort(__float2half_rn(v))
+                               : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+// 8 sums (bias included) of row m, features n .. n + 7, to outputs.
+template <bool BF, int ODT>
+__device__ __forceinline__ void finish8(const LinParams &p, float (&z)[8], const Operands &o,
+                                        uint32_t m, uint32_t n) {
     switch (p.act) {
-        case HCT_B200_ACT_RELU: activate16<HCT_B200_ACT_RELU>(z); break;
-        case HCT_B200_ACT_SILU: activate16<HCT_B200_ACT_SILU>(z); break;
-        case HCT_B200_ACT_GELU: activate16<HCT_B200_ACT_GELU>(z); break;
-        case HCT_B200_ACT_GELU_TANH: activate16<HCT_B200_ACT_GELU_TANH>(z); break;
+        case HCT_B200_ACT_RELU: activate_all<HCT_B200_ACT_RELU>(z); break;
+        case HCT_B200_ACT_SILU: activate_all<HCT_B200_ACT_SILU>(z); break;
+        case HCT_B200_ACT_GELU: activate_all<HCT_B200_ACT_GELU>(z); break;
+        case HCT_B200_ACT_GELU_TANH: activate_all<HCT_B200_ACT_GELU_TANH>(z); break;
         default: break;
     }
     if (p.gate) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) z[j] *= g[j];
+        for (int j = 0; j < 8; j++) z[j] *= from16<BF>((uint16_t)(o.g[j / 2] >> (16 * (j & 1))));
     }
     if (p.res) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) z[j] += r[j];
+        for (int j = 0; j < 8; j++)
+            z[j] += ODT == HCT_B200_F32
+                        ? __uint_as_float(o.r[j])
+                        : from16<ODT == HCT_B200_BF16>((uint16_t)(o.r[j / 2] >> (16 * (j & 1))));
     }
     const uint64_t at = (uint64_t)m * p.ldo + n;
+    const bool whole = n + 8 <= p.N && p.vec_out;
+    if (ODT == HCT_B200_F32) {
+        float *q = reinterpret_cast<float *>(p.out) + at;
+        if (whole) {
+            reinterpret_cast<float4 *>(q)[0] = make_float4(z[0], z[1], z[2], z[3]);
+            reinterpret_cast<float4 *>(q)[1] = make_float4(z[4], z[5], z[6], z[7]);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 16; j++)
-        if (j < (int)count) store_out(p.out, at + (uint64_t)j * p.ldo, ODT, z[j]);
+            for (int j = 0; j < 8; j++)
+                if (n + j < p.N) q[j] = z[j];
+        }
+    } else {
+        uint16_t *q = reinterpret_cast<uint16_t *>(p.out) + at;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = to16<ODT>(z[2 * j]) | to16<ODT>(z[2 * j + 1]) << 16;
+        if (whole) {
+            *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (n + j < p.N) q[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+        }
+    }
+}
+template <bool BF, bool PRECISE>
+__device__ __forceinline__ void finish8_any(const LinParams &p, float (&z)[8], const Operands &o,
+                                            uint32_t m, uint32_t n) {
+    if (PRECISE) finish8<BF, HCT_B200_F32>(p, z, o, m, n);
+    else if (p.odt == HCT_B200_F16) finish8<BF, HCT_B200_F16>(p, z, o, m, n);
+    else finish8<BF, HCT_B200_BF16>(p, z, o, m, n);
 }
 
-constexpr int umma_threads(bool int4) { return int4 ? 512 : 256; }
+// Sixteen rows m .. m + 15 (count of them live) of a tile's 128 features, a
+// feature per thread of the set in z: through the set's shared memory (16 x
+// 128 floats) to its threads by rows, each 2 rows x 8 features n .. n + 7.
+template <bool BF, bool PRECISE>
+__device__ __forceinline__ void finish_rows(const LinParams &p, const float (&z)[16], float *stage,
+                                            uint32_t set, uint32_t id, const float (&bias)[8],
+                                            uint32_t m, uint32_t count, uint32_t n) {
+    Operands o[2];
+    const uint32_t j0 = id / 16;
+    const bool live = n < p.N;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (live && j0 + 8 * i < count) load_operands<PRECISE ? HCT_B200_F32 : HCT_B200_F16>(p, m + j0 + 8 * i, n, o[i]);
+    asm volatile("bar.sync %0, 128;" ::"r"(set + 1) : "memory");  // the last rows have been read
+#pragma unroll
+    for (int j = 0; j < 16; j++) stage[j * 128 + id] = z[j];
+    asm volatile("bar.sync %0, 128;" ::"r"(set + 1) : "memory");
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (!live || j0 + 8 * i >= count) continue;
+        const float4 *q = reinterpret_cast<const float4 *>(stage + (j0 + 8 * i) * 128 + id % 16 * 8);
+        const float4 a = q[0], b = q[1];
+        float v[8] = {a.x + bias[0], a.y + bias[1], a.z + bias[2], a.w + bias[3],
+                      b.x + bias[4], b.y + bias[5], b.z + bias[6], b.w + bias[7]};
+        finish8_any<BF, PRECISE>(p, v, o[i], m + j0 + 8 * i, n);
+    }
+}
+
+template <bool BF>
+__device__ __forceinline__ void load_bias8(const LinParams &p, uint32_t e, uint32_t n,
+                                           float (&bias)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) bias[j] = n + j < p.N ? bias_of<BF>(p, e, n + j) : 0.0f;
+}
+
+constexpr int umma_threads(bool int4) { return int4 ? 768 : 384; }
+// rows per tile at most: a thread of the epilogue keeps half of them as f32 sums where PRECISE
+__host__ __device__ constexpr uint32_t max_rows(bool int4, bool precise) { return precise ? (int4 ? 64 : 128) : 256; }
 
 template <bool INT4, bool BF, bool PRECISE>
 __global__ void __launch_bounds__(umma_threads(INT4), 1)
     linear_umma_kernel(const __grid_constant__ CUtensorMap tmX,
                        const __grid_constant__ CUtensorMap tmW, const __grid_constant__ UmmaParams u) {
     constexpr uint32_t A_PARTS = INT4 && PRECISE ? 2 : 1;
-    constexpr int GROUPS = 2;  // of dequantising warps
+    constexpr uint32_t GROUPS = 3;  // of dequantising warps
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const LinParams &p = u.p;
     const uint32_t stages = u.stages, stage_bytes = A_PARTS * A_BYTES + u.bn * 128;
     uint8_t *raw = smem + (size_t)stages * stage_bytes;
-    Ctl *ctl = reinterpret_cast<Ctl *>(raw + (size_t)u.raw_stages * PK_BYTES);
+    uint8_t *epi = raw + (size_t)u.raw_stages * PK_BYTES;
+    Ctl *ctl = reinterpret_cast<Ctl *>(epi + EPI_BYTES);
     uint32_t *first = reinterpret_cast<uint32_t *>(ctl + 1), *off = first + p.E + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -589,7 +730,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(smem_u32(&ctl->tfull[b]), 1);
-            mbar_init(smem_u32(&ctl->tempty[b]), 4);
+            mbar_init(smem_u32(&ctl->tempty[b]), 8);
         }
         mbar_init(smem_u32(&ctl->drain), 1);
         ctl->abort = 0;
@@ -631,25 +772,24 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
             if (!INT4)
                 asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW))
                              : "memory");
-            uint32_t it = 0;
+            Ring at(stages);
             bool ok = true;
             for (uint32_t t = t0; ok && t < tiles; t += step) {
                 const Tile c = tile_at(u, first, off, t);
                 const uint32_t boxes = (c.rows + u.xbox - 1) / u.xbox;
-                for (uint32_t kb = kb0; kb < kb1; kb++, it++) {
-                    const uint32_t s = it % stages, ph = (it / stages) & 1u;
-                    if (aborted() || !mbar_wait(smem_u32(&ctl->empty[s]), ph ^ 1u)) {
+                for (uint32_t kb = kb0; kb < kb1; kb++, at.step()) {
+                    if (aborted() || !mbar_wait(smem_u32(&ctl->empty[at.slot]), at.pass ^ 1u)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t sa = smem_u32(smem + (size_t)s * stage_bytes);
-                    const uint32_t sb = sa + A_PARTS * A_BYTES, fb = smem_u32(&ctl->xfull[s]);
+                    const uint32_t sa = smem_u32(smem + (size_t)at.slot * stage_bytes);
+                    const uint32_t sb = sa + A_PARTS * A_BYTES, fb = smem_u32(&ctl->xfull[at.slot]);
                     mbar_expect_tx(fb, boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES));
                     if (!INT4) tma_3d(sa, &tmW, fb, (int)(kb * BK), (int)c.n0, (int)c.e);
                     for (uint32_t b = 0; b < boxes; b++)
                         tma_2d(sb + b * u.xbox * 128, &tmX, fb, (int)(kb * BK),
                                (int)(c.m0 + b * u.xbox));
-                    *(volatile int *)&ctl->issued = (int)(it + 1);
+                    *(volatile int *)&ctl->issued = *(volatile int *)&ctl->issued + 1;
                 }
             }
             if (!ok) give_up();
@@ -658,28 +798,27 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         if (lane == 0) {
             // D = F32, A = B = x's type, both K-major, M = 128; N follows the tile
             const uint32_t idesc0 = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);
-            uint32_t it = 0, use = 0;
+            Ring at(stages), acc(2);
             bool ok = true;
             for (uint32_t t = t0; ok && t < tiles; t += step) {
                 const Tile c = tile_at(u, first, off, t);
                 const uint32_t idesc = idesc0 | ((c.rows + 15) / 16 * 2) << 17;
-                for (uint32_t kb = kb0; ok && kb < kb1; use++) {
-                    const uint32_t end = min(kb + sect, kb1), buf = use & 1u;
-                    if (!mbar_wait(smem_u32(&ctl->tempty[buf]), ((use >> 1) & 1u) ^ 1u)) {
+                for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
+                    const uint32_t end = min(kb + sect, kb1);
+                    if (!mbar_wait(smem_u32(&ctl->tempty[acc.slot]), acc.pass ^ 1u)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d = tmem + buf * u.tmem_stride;
-                    for (uint32_t from = kb; kb < end; kb++, it++) {
-                        const uint32_t s = it % stages, ph = (it / stages) & 1u;
-                        if (aborted() || !mbar_wait(smem_u32(&ctl->xfull[s]), ph) ||
-                            (INT4 && !mbar_wait(smem_u32(&ctl->afull[s]), ph))) {
+                    const uint32_t d = tmem + acc.slot * u.tmem_stride;
+                    for (uint32_t from = kb; kb < end; kb++, at.step()) {
+                        if (aborted() || !mbar_wait(smem_u32(&ctl->xfull[at.slot]), at.pass) ||
+                            (INT4 && !mbar_wait(smem_u32(&ctl->afull[at.slot]), at.pass))) {
                             ok = false;
                             break;
                         }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = smem_u32(smem + (size_t)s * stage_bytes);
+                        const uint32_t sa = smem_u32(smem + (size_t)at.slot * stage_bytes);
                         const uint64_t db = umma_desc(sa + A_PARTS * A_BYTES);
 #pragma unroll
                         for (uint32_t a = 0; a < A_PARTS; a++) {
@@ -688,9 +827,9 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                             for (uint32_t k = 0; k < BK / 16; k++)
                                 umma(d, da + 2 * k, db + 2 * k, idesc, kb != from || a || k);
                         }
-                        umma_commit(smem_u32(&ctl->empty[s]));
+                        umma_commit(smem_u32(&ctl->empty[at.slot]));
                     }
-                    if (ok) umma_commit(smem_u32(&ctl->tfull[buf]));
+                    if (ok) umma_commit(smem_u32(&ctl->tfull[acc.slot]));
                 }
             }
             if (!ok) give_up();
@@ -699,151 +838,138 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     } else if (INT4 && warp == 3) {
         if (lane == 0) {
             const uint64_t per_expert = (uint64_t)nt * kbs;
-            uint32_t it = 0;
+            Ring at(u.raw_stages);
             bool ok = true;
             for (uint32_t t = t0; ok && t < tiles; t += step) {
                 const Tile c = tile_at(u, first, off, t);
                 const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
                                      (c.e * per_expert + (uint64_t)(c.n0 / 128) * kbs + kb0) * PK_BYTES;
-                for (uint32_t kb = kb0; kb < kb1; kb++, it++, src += PK_BYTES) {
-                    const uint32_t r = it % u.raw_stages, ph = (it / u.raw_stages) & 1u;
-                    if (aborted() || !mbar_wait(smem_u32(&ctl->rempty[r]), ph ^ 1u)) {
+                for (uint32_t kb = kb0; kb < kb1; kb++, at.step(), src += PK_BYTES) {
+                    if (aborted() || !mbar_wait(smem_u32(&ctl->rempty[at.slot]), at.pass ^ 1u)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t fb = smem_u32(&ctl->rfull[r]);
+                    const uint32_t fb = smem_u32(&ctl->rfull[at.slot]);
                     mbar_expect_tx(fb, PK_BYTES);
-                    bulk_load(smem_u32(raw + (size_t)r * PK_BYTES), src, PK_BYTES, fb);
-                    *(volatile int *)&ctl->raw_issued = (int)(it + 1);
+                    bulk_load(smem_u32(raw + (size_t)at.slot * PK_BYTES), src, PK_BYTES, fb);
+                    *(volatile int *)&ctl->raw_issued = *(volatile int *)&ctl->raw_issued + 1;
                 }
             }
             if (!ok) give_up();
         }
-    } else if (INT4 && warp >= 8) {
-        const uint32_t group = (warp - 8) >> 2, row = threadIdx.x & 127u;
-        uint32_t it = 0;
-        bool ok = true;
-        for (uint32_t t = t0; ok && t < tiles; t += step) {
-            for (uint32_t kb = kb0; kb < kb1; kb++, it++) {
-                if (it % GROUPS != group) continue;
-                const uint32_t r = it % u.raw_stages, s = it % stages;
-                if (aborted() || !mbar_wait(smem_u32(&ctl->rfull[r]), (it / u.raw_stages) & 1u)) {
-                    ok = false;
-                    break;
-                }
-                const uint8_t *src = raw + (size_t)r * PK_BYTES;
-                uint4 q[2];
-                uint16_t sc[2];
+    } else if (INT4 && warp >= 12) {
+        // this group's K steps of all the CTA's tiles, one after another
+        const uint32_t group = (warp - 12) >> 2, row = threadIdx.x & 127u;
+        const uint64_t steps = t0 < tiles ? (uint64_t)((tiles - t0 - 1) / step + 1) * (kb1 - kb0) : 0;
+        Ring in(u.raw_stages, group), to(stages, group);
+        const uint32_t mine = row * 128 + ((row & 7u) << 4);  // chunk c of my row: ^ (c << 4)
+        for (uint64_t it = group; it < steps; it += GROUPS, in.step(GROUPS), to.step(GROUPS)) {
+            if (aborted() || !mbar_wait(smem_u32(&ctl->rfull[in.slot]), in.pass)) {
+                give_up();
+                break;
+            }
+            const uint8_t *src = raw + (size_t)in.slot * PK_BYTES;
+            uint4 q[2];
+            uint16_t sc[2];
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    q[g] = *reinterpret_cast<const uint4 *>(src + (g * 128 + row) * 16);
-                    sc[g] = *reinterpret_cast<const uint16_t *>(src + PK_NIB + (g * 128 + row) * 2);
-                }
-                if (!mbar_wait(smem_u32(&ctl->empty[s]), ((it / stages) & 1u) ^ 1u)) {
-                    ok = false;
-                    break;
-                }
-                uint8_t *a = smem + (size_t)s * stage_bytes + row * 128;
+            for (int g = 0; g < 2; g++) {
+                q[g] = *reinterpret_cast<const uint4 *>(src + (g * 128 + row) * 16);
+                sc[g] = *reinterpret_cast<const uint16_t *>(src + PK_NIB + (g * 128 + row) * 2);
+            }
+            if (!mbar_wait(smem_u32(&ctl->empty[to.slot]), to.pass ^ 1u)) {
+                give_up();
+                break;
+            }
+            uint8_t *a = smem + (size_t)to.slot * stage_bytes;
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const Scale<BF> scale(sc[g]);
-                    const uint32_t w[4] = {q[g].x, q[g].y, q[g].z, q[g].w};
+            for (int g = 0; g < 2; g++) {
+                const Scale<BF> scale(sc[g]);
+                const uint32_t w[4] = {q[g].x, q[g].y, q[g].z, q[g].w};
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t v[4], l[4];
-                        dequant8<PRECISE>(w[c], scale, v, l);
-                        uint8_t *o = a + (((g * 4 + c) ^ (row & 7u)) << 4);
-                        *reinterpret_cast<uint4 *>(o) = make_uint4(v[0], v[1], v[2], v[3]);
-                        if (PRECISE)
-                            *reinterpret_cast<uint4 *>(o + A_BYTES) = make_uint4(l[0], l[1], l[2], l[3]);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&ctl->afull[s]));
-                    mbar_arrive(smem_u32(&ctl->rempty[r]));
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[4], l[4];
+                    dequant8<PRECISE>(w[c], scale, v, l);
+                    uint8_t *o = a + (mine ^ ((g * 4 + c) << 4));
+                    *reinterpret_cast<uint4 *>(o) = make_uint4(v[0], v[1], v[2], v[3]);
+                    if (PRECISE)
+                        *reinterpret_cast<uint4 *>(o + A_BYTES) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&ctl->afull[to.slot]));
+                mbar_arrive(smem_u32(&ctl->rempty[in.slot]));
+            }
         }
-        if (!ok) give_up();
-    } else if (warp >= 4 && warp < 8) {
-        const uint32_t q = warp & 3u, row = q * 32 + lane;
+    } else if (warp >= 4 && warp < 12) {
+        constexpr int CHUNKS = max_rows(INT4, PRECISE) / 32;  // of 16 rows, per set
+        const uint32_t set = (warp - 4) >> 2, q = warp & 3u, id = q * 32 + lane;
         float *part = reinterpret_cast<float *>(smem);  // split: [rows of x][128 features]
-        uint32_t use = 0;
+        float *stage = reinterpret_cast<float *>(epi + set * (EPI_BYTES / 2));
+        Ring acc(2);
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
             const Tile c = tile_at(u, first, off, t);
-            const uint32_t n = c.n0 + row;
-            const bool live = n < p.N;
-            const float bias = live && u.split == 1 ? bias_of<BF>(p, c.e, n) : 0.0f;
-            if (!PRECISE) {
-                const uint32_t buf = use & 1u;
-                if (!mbar_wait(smem_u32(&ctl->tfull[buf]), (use >> 1) & 1u) || aborted()) {
+            const uint32_t n = c.n0 + id % 16 * 8;
+            float bias[8];
+            if (u.split == 1) load_bias8<BF>(p, c.e, n, bias);
+            float sum[PRECISE ? CHUNKS : 1][16];
+            if (PRECISE) {
+#pragma unroll
+                for (int i = 0; i < (PRECISE ? CHUNKS : 1); i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) sum[i][j] = 0.0f;
+            }
+            for (uint32_t kb = kb0; kb < kb1; kb += sect, acc.step()) {
+                if (!mbar_wait(smem_u32(&ctl->tfull[acc.slot]), acc.pass) || aborted()) {
                     ok = false;
                     break;
                 }
-                use++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t ta = tmem + buf * u.tmem_stride + ((q * 32) << 16);
-                for (uint32_t j0 = 0; j0 < c.rows; j0 += 16) {
-                    uint32_t v[16];
-                    float z[16];
-                    __syncwarp();
-                    tmem_ld16(ta + j0, v);
+                const uint32_t ta = tmem + acc.slot * u.tmem_stride + ((q * 32) << 16);
+                if (PRECISE) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) z[j] = __uint_as_float(v[j]);
-                    if (u.split > 1) {
+                    for (int i = 0; i < (PRECISE ? CHUNKS : 1); i++) {
+                        const uint32_t j0 = (2 * i + set) * 16;
+                        if (j0 >= c.rows) continue;
+                        uint32_t v[16];
+                        __syncwarp();
+                        tmem_ld16(ta + j0, v);
 #pragma unroll
-                        for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + row] = z[j];
-                    } else if (live) {
-                        const uint32_t count = min(16u, c.rows - j0);
-                        if (p.odt == HCT_B200_F16)
-                            finish16<BF, HCT_B200_F16>(p, z, bias, c.m0 + j0, count, n);
-                        else
-                            finish16<BF, HCT_B200_BF16>(p, z, bias, c.m0 + j0, count, n);
+                        for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
+                    }
+                } else {
+                    for (uint32_t j0 = set * 16; j0 < c.rows; j0 += 32) {
+                        uint32_t v[16];
+                        float z[16];
+                        __syncwarp();
+                        tmem_ld16(ta + j0, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) z[j] = __uint_as_float(v[j]);
+                        if (u.split > 1) {
+#pragma unroll
+                            for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + id] = z[j];
+                        } else {
+                            finish_rows<BF, false>(p, z, stage, set, id, bias, c.m0 + j0,
+                                                   c.rows - j0, n);
+                        }
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[buf]));
-            } else {
-                float z[PRECISE_BN / 16][16];
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[acc.slot]));
+            }
+            if (PRECISE && ok) {
 #pragma unroll
-                for (int i = 0; i < PRECISE_BN / 16; i++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) z[i][j] = 0.0f;
-                for (uint32_t kb = kb0; kb < kb1; kb += sect, use++) {
-                    const uint32_t buf = use & 1u;
-                    if (!mbar_wait(smem_u32(&ctl->tfull[buf]), (use >> 1) & 1u) || aborted()) {
-                        ok = false;
-                        break;
-                    }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t ta = tmem + buf * u.tmem_stride + ((q * 32) << 16);
-#pragma unroll
-                    for (int i = 0; i < PRECISE_BN / 16; i++) {
-                        if (i * 16 >= (int)c.rows) continue;
-                        uint32_t v[16];
-                        __syncwarp();
-                        tmem_ld16(ta + i * 16, v);
-#pragma unroll
-                        for (int j = 0; j < 16; j++) z[i][j] += __uint_as_float(v[j]);
-                    }
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[buf]));
-                }
-                if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < PRECISE_BN / 16; i++) {
-                    if (i * 16 >= (int)c.rows) continue;
+                for (int i = 0; i < (PRECISE ? CHUNKS : 1); i++) {
+                    const uint32_t j0 = (2 * i + set) * 16;
+                    if (j0 >= c.rows) continue;
                     if (u.split > 1) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) part[(i * 16 + j) * 128 + row] = z[i][j];
-                    } else if (live) {
-                        finish16<BF, HCT_B200_F32>(p, z[i], bias, c.m0 + i * 16,
-                                                   min(16u, c.rows - i * 16), n);
+                        for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + id] = sum[i][j];
+                    } else {
+                        finish_rows<BF, true>(p, sum[i], stage, set, id, bias, c.m0 + j0, c.rows - j0, n);
                     }
                 }
             }
@@ -860,14 +986,23 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         if (t0 < tiles && !aborted()) {
             const Tile c = tile_at(u, first, off, t0);
             const uint32_t j0 = c.rows * rank / u.split, j1 = c.rows * (rank + 1) / u.split;
-            const uint32_t f = threadIdx.x & 127u, n = c.n0 + f;
-            const uint32_t base = smem_u32(smem);
+            const uint32_t f = threadIdx.x % 16 * 8, n = c.n0 + f, base = smem_u32(smem);
             if (n < p.N) {
-                const float bias = bias_of<BF>(p, c.e, n);
-                for (uint32_t j = j0 + threadIdx.x / 128; j < j1; j += blockDim.x / 128) {
-                    float z = 0.0f;
-                    for (uint32_t r = 0; r < u.split; r++) z += ld_cluster(base + (j * 128 + f) * 4, r);
-                    finish<BF>(p, c.m0 + j, n, z + bias);
+                float bias[8];
+                load_bias8<BF>(p, c.e, n, bias);
+                for (uint32_t j = j0 + threadIdx.x / 16; j < j1; j += blockDim.x / 16) {
+                    Operands o;
+                    load_operands<PRECISE ? HCT_B200_F32 : HCT_B200_F16>(p, c.m0 + j, n, o);
+                    float z[8] = {};
+                    for (uint32_t r = 0; r < u.split; r++) {
+                        const float4 a = ld_cluster(base + (j * 128 + f) * 4, r);
+                        const float4 b = ld_cluster(base + (j * 128 + f + 4) * 4, r);
+                        z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
+                        z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) z[i] += bias[i];
+                    finish8_any<BF, PRECISE>(p, z, o, c.m0 + j, n);
                 }
             }
         }
@@ -1045,9 +1180,16 @@ template <bool INT4, bool BF, bool PRECISE>
 cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const UmmaParams &u,
                         uint32_t grid, uint32_t smem, cudaStream_t s) {
     const auto kernel = linear_umma_kernel<INT4, BF, PRECISE>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)SMEM_LIMIT);
+    // once per device (64 of them remembered); twice by two threads does no harm
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(grid);
     c.blockDim = dim3(umma_threads(INT4));
@@ -1065,7 +1207,7 @@ cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const Umma
 // Tile height, split and ring depths of a call on the tensor-core kernel.
 cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaStream_t s) {
     const bool precise = p.odt == HCT_B200_F32;
-    const uint32_t sms = (uint32_t)sm_count(), cap = precise ? PRECISE_BN : 256;
+    const uint32_t sms = (uint32_t)sm_count(), cap = max_rows(int4, precise);
     const uint32_t nt = (p.N + 127) / 128, kbs = (p.K + BK - 1) / BK;
     UmmaParams u{};
     u.p = p;
@@ -1107,7 +1249,8 @@ cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaS
     while (u.tmem_cols < 2 * u.tmem_stride) u.tmem_cols *= 2;
     const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn * 128;
     u.raw_stages = int4 ? 10 : 0;
-    const uint32_t fixed = 1024 + u.raw_stages * PK_BYTES + (uint32_t)sizeof(Ctl) + (p.E + 1) * 8;
+    const uint32_t fixed =
+        1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) + (p.E + 1) * 8;
     u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
     const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
 
@@ -1159,6 +1302,13 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     p.bias_f32 = a->bias_dtype == HCT_B200_F32;
     p.act = a->activation;
     p.odt = a->out_dtype;
+    const auto rows16 = [&](const void *q, uint64_t ld, uint64_t size) {
+        return (uintptr_t)q % 16 == 0 && (p.M == 1 || ld * size % 16 == 0);
+    };
+    const uint64_t osz = p.odt == HCT_B200_F32 ? 4 : 2;
+    p.vec_gate = rows16(p.gate, p.ldgate, 2);
+    p.vec_res = rows16(p.res, p.ldres, osz);
+    p.vec_out = rows16(p.out, p.ldo, osz);
     const bool bf = a->x_dtype == HCT_B200_BF16, int4 = a->weight_form == HCT_B200_WEIGHT_INT4;
     // the tensor cores take rows that TMA can fetch (and strides that its maps can hold)
     const bool w_ok = int4 || (tma_rows(p.w, p.N, p.ldw, p.K) &&

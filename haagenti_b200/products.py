@@ -19,13 +19,17 @@ __all__ = ["Int4Weight", "linear", "grouped_linear", "linear_status"]
 
 _TAG: dict = {}   # torch dtype -> F32 / F16 / BF16
 _TYPE: dict = {}  # and back
+_raw_stream = None  # device index -> its current stream's cudaStream_t
 
 
-def _types():
+def _first_call():
+    global _raw_stream
     torch = _torch()
+    # the handle alone: torch.cuda.current_stream builds a Stream object, 3 us of a call's 10
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                          lambda i: torch.cuda.current_stream(i).cuda_stream)
     _TAG.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
     _TYPE.update({v: k for k, v in _TAG.items()})
-    return _TAG
 
 
 class Int4Weight:
@@ -88,31 +92,32 @@ class Int4Weight:
         return s if self.experts is None else (self.experts,) + s
 
 
-def _matrix(t, name, shape, dtype, device):
+def _matrix(t, name, shape, dtype, dev):
     """Row stride of an optional (rows, features) operand after its checks."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, x on {device}")
-    s = t.stride()
-    if s[1] != 1 and shape[1] > 1:
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {shape} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, x on cuda:{dev}")
+    ld, step = t.stride()
+    if step != 1 and shape[1] > 1:
         raise ValueError(f"the features of {name} must be contiguous")
-    return s[0]
+    return ld
 
 
 def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, out, stream):
     torch = _torch()
-    tags = _TAG or _types()
+    if not _TAG:
+        _first_call()
     if x.dim() != 2 or not x.is_cuda:
         raise ValueError("x must be a 2-D CUDA tensor (rows, in_features)")
-    device = x.device
+    dev = x.get_device()
     m, k = x.shape
     xt = x.dtype
-    x_tag = tags.get(xt)
-    if x_tag is None or x_tag == F32:
+    x_tag = _TAG.get(xt)
+    if not x_tag:  # no type of ours, or F32 (0)
         raise ValueError(f"x must be float16 or bfloat16, got {xt}")
-    sx = x.stride()
-    if sx[1] != 1 and k > 1:
+    ldx, step = x.stride()
+    if step != 1 and k > 1:
         raise ValueError("the features of x must be contiguous")
     ldw = w_stride = 0
     experts = None
@@ -127,34 +132,34 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
         if weight.dim() != (2 if offsets is None else 3):
             raise ValueError("a dense weight is (out_features, in_features), with a leading axis "
                              "of experts in grouped_linear")
-        n, wk = weight.shape[-2:]
-        ws = weight.stride()
-        if ws[-1] != 1 and wk > 1:
+        if offsets is None:
+            n, wk = weight.shape
+            ldw, step = weight.stride()
+        else:
+            experts, n, wk = weight.shape
+            w_stride, ldw, step = weight.stride()
+        if step != 1 and wk > 1:
             raise ValueError("the input features of a dense weight must be contiguous")
-        ldw = ws[-2]
-        if offsets is not None:
-            experts, w_stride = weight.shape[0], ws[0]
     if wk != k:
         raise ValueError(f"x has {k} features, the weight {wk}")
-    if wt.device != device:
-        raise ValueError(f"the weight is on {wt.device}, x on {device}")
-    bits = 32
+    if wt.get_device() != dev:
+        raise ValueError(f"the weight is on {wt.device}, x on {x.device}")
+    bits, off_ptr = 32, None
     if offsets is None:
         if experts is not None:
             raise ValueError("a weight with experts needs grouped_linear")
         experts = 0
-        off_ptr = None
     else:
         if experts is None:
             raise ValueError("grouped_linear needs a weight with experts (an Int4Weight of a list)")
-        if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != device:
+        if offsets.dtype not in (torch.int32, torch.int64) or offsets.get_device() != dev:
             raise ValueError("offsets must be an int32 or int64 tensor on x's device")
         if offsets.dim() != 1 or offsets.shape[0] != experts + 1 or not offsets.is_contiguous():
             raise ValueError(f"offsets must hold experts + 1 = {experts + 1} contiguous values")
         bits = 32 if offsets.dtype == torch.int32 else 64
         off_ptr = offsets.data_ptr()
     if out is not None:
-        tag = tags.get(out.dtype)
+        tag = _TAG.get(out.dtype)
         if tag is None or (out_dtype is not None and out_dtype != tag):
             raise ValueError(f"out is of {out.dtype}, not of out_dtype {out_dtype}")
     else:
@@ -163,46 +168,47 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
             raise ValueError(f"out_dtype must be F32, F16 or BF16, got {out_dtype}")
     ot = _TYPE[tag]
     shape = (m, n)
-    bias_tag = x_tag
+    bias_tag, bias_ptr, gate_ptr, res_ptr, ldg, ldr = x_tag, None, None, None, 0, 0
+    grads = x.requires_grad or wt.requires_grad
     if bias is not None:
         want = (n,) if offsets is None else (experts, n)
-        bias_tag = tags.get(bias.dtype)
-        if (bias_tag != x_tag and bias_tag != F32) or tuple(bias.shape) != want:
+        bias_tag = _TAG.get(bias.dtype)
+        if (bias_tag != x_tag and bias_tag != F32) or bias.shape != want:
             raise ValueError(f"bias must be {want} of {xt} or float32, got {tuple(bias.shape)} of "
                              f"{bias.dtype}")
-        if bias.device != device or not bias.is_contiguous():
+        if bias.get_device() != dev or not bias.is_contiguous():
             raise ValueError("bias must be contiguous and on x's device")
-    ldg = _matrix(gate, "gate", shape, xt, device) if gate is not None else 0
-    ldr = _matrix(residual, "residual", shape, ot, device) if residual is not None else 0
+        bias_ptr = bias.data_ptr()
+        grads |= bias.requires_grad
+    if gate is not None:
+        ldg, gate_ptr = _matrix(gate, "gate", shape, xt, dev), gate.data_ptr()
+        grads |= gate.requires_grad
+    if residual is not None:
+        ldr, res_ptr = _matrix(residual, "residual", shape, ot, dev), residual.data_ptr()
+        grads |= residual.requires_grad
     if out is not None:
-        _matrix(out, "out", shape, ot, device)
-    if torch.is_grad_enabled():
-        for t in (x, weight, bias, gate, residual, out):
-            if t is not None and getattr(t, "requires_grad", False):
-                raise Unsupported(L.UNSUPPORTED, "the products have no backward pass: detach the "
-                                                 "tensors or call under torch.no_grad()")
+        _matrix(out, "out", shape, ot, dev)
+        grads |= out.requires_grad
+    if grads and torch.is_grad_enabled():
+        raise Unsupported(L.UNSUPPORTED, "the products have no backward pass: detach the tensors "
+                                         "or call under torch.no_grad()")
     lib = L.load()
     fn = lib.hct_b200_linear if offsets is None else lib.hct_b200_grouped_linear
 
     def call(raw):
-        o = out if out is not None else torch.empty(shape, dtype=ot, device=device)
-        args = L.LinearArgs(
-            m, n, k, x.data_ptr(), sx[0], wt.data_ptr(), ldw, w_stride,
-            None if bias is None else bias.data_ptr(),
-            None if gate is None else gate.data_ptr(), ldg,
-            None if residual is None else residual.data_ptr(), ldr,
-            o.data_ptr(), o.stride(0), off_ptr, experts, bits, x_tag, form, bias_tag, tag,
-            activation, 0)
-        _check(fn(args, raw))
+        o = out if out is not None else torch.empty(shape, dtype=ot, device=x.device)
+        _check(fn(L.LinearArgs(m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride, bias_ptr,
+                               gate_ptr, ldg, res_ptr, ldr, o.data_ptr(), o.stride(0), off_ptr,
+                               experts, bits, x_tag, form, bias_tag, tag, activation, 0), raw))
         return o
 
-    if stream is None and torch.cuda.current_device() == device.index:
-        return call(torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(device):
+    if stream is None and torch.cuda.current_device() == dev:
+        return call(_raw_stream(dev))
+    with torch.cuda.device(dev):
         if stream is None or stream == torch.cuda.current_stream():
-            return call(torch.cuda.current_stream().cuda_stream)
-        if stream.device != device:
-            raise ValueError(f"the stream belongs to {stream.device}, x to {device}")
+            return call(_raw_stream(dev))
+        if stream.device.index != dev:
+            raise ValueError(f"the stream belongs to {stream.device}, x to {x.device}")
         with torch.cuda.stream(stream):
             o = call(stream.cuda_stream)
         # the caller's tensors are read on a stream that their allocator does not know of
