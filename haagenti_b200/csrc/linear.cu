@@ -356,19 +356,47 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait (2 s): false when the phase did not complete in time.  The
-// clock is read only once the wait has become a long one.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+// Bounded wait (2 s): false when the phase did not complete in time or the CTA
+// has given up meanwhile.  The clock is read only once the wait is a long one.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const int *abort) {
     uint64_t t0 = 0;
     for (uint32_t i = 1; i < (1u << 30); ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 0) {
+            if (*(const volatile int *)abort) return false;
             const uint64_t t = globaltimer();
             if (t0 == 0) t0 = t;
             else if (t - t0 > 2000000000ull) return false;
         }
     }
     return false;
+}
+// The same by a whole warp: true when every lane's phase completed.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const int *abort) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+}
+// Whether every one of the 128 threads of an epilogue set says ok, so that all of
+// them go on to its barriers or none does.
+__device__ __forceinline__ bool set_agrees(uint32_t set, bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)ok), "r"(set + 1)
+        : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e != 0;
 }
 
 // A position in a ring of slots: the slot and the parity of its current pass.
@@ -766,97 +794,97 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     const uint32_t kb1 = (uint32_t)((uint64_t)kbs * (rank + 1) / u.split);
     const uint32_t sect = PRECISE ? SECTION : kb1 - kb0;  // K steps per accumulation
 
+    // The producers and the MMA warp run whole (their addresses and descriptors
+    // are warp-uniform); one elected lane issues.
     if (warp == 0) {
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
-            if (!INT4)
-                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW))
-                             : "memory");
-            Ring at(stages);
-            bool ok = true;
-            for (uint32_t t = t0; ok && t < tiles; t += step) {
-                const Tile c = tile_at(u, first, off, t);
-                const uint32_t boxes = (c.rows + u.xbox - 1) / u.xbox;
-                for (uint32_t kb = kb0; kb < kb1; kb++, at.step()) {
-                    if (aborted() || !mbar_wait(smem_u32(&ctl->empty[at.slot]), at.pass ^ 1u)) {
-                        ok = false;
-                        break;
-                    }
+        Ring at(stages);
+        uint32_t issued = 0;
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += step) {
+            const Tile c = tile_at(u, first, off, t);
+            const uint32_t boxes = (c.rows + u.xbox - 1) / u.xbox;
+            const uint32_t bytes = boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES);
+            for (uint32_t kb = kb0; kb < kb1; kb++, at.step()) {
+                ok = mbar_wait_warp(smem_u32(&ctl->empty[at.slot]), at.pass ^ 1u, &ctl->abort);
+                if (!ok) break;
+                if (elect_one()) {
                     const uint32_t sa = smem_u32(smem + (size_t)at.slot * stage_bytes);
                     const uint32_t sb = sa + A_PARTS * A_BYTES, fb = smem_u32(&ctl->xfull[at.slot]);
-                    mbar_expect_tx(fb, boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES));
+                    mbar_expect_tx(fb, bytes);
                     if (!INT4) tma_3d(sa, &tmW, fb, (int)(kb * BK), (int)c.n0, (int)c.e);
                     for (uint32_t b = 0; b < boxes; b++)
                         tma_2d(sb + b * u.xbox * 128, &tmX, fb, (int)(kb * BK),
                                (int)(c.m0 + b * u.xbox));
-                    *(volatile int *)&ctl->issued = *(volatile int *)&ctl->issued + 1;
                 }
+                __syncwarp();
+                issued++;
             }
-            if (!ok) give_up();
         }
+        if (lane == 0) ctl->issued = (int)issued;
+        if (!ok) give_up();
     } else if (warp == 1) {
-        if (lane == 0) {
-            // D = F32, A = B = x's type, both K-major, M = 128; N follows the tile
-            const uint32_t idesc0 = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);
-            Ring at(stages), acc(2);
-            bool ok = true;
-            for (uint32_t t = t0; ok && t < tiles; t += step) {
-                const Tile c = tile_at(u, first, off, t);
-                const uint32_t idesc = idesc0 | ((c.rows + 15) / 16 * 2) << 17;
-                for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
-                    const uint32_t end = min(kb + sect, kb1);
-                    if (!mbar_wait(smem_u32(&ctl->tempty[acc.slot]), acc.pass ^ 1u)) {
-                        ok = false;
-                        break;
-                    }
+        // D = F32, A = B = x's type, both K-major, M = 128; N follows the tile
+        const uint32_t idesc0 = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);
+        // INT4: half of the lanes wait for the x tile, half for the weights
+        const uint32_t full = smem_u32(INT4 && lane >= 16 ? ctl->afull : ctl->xfull);
+        Ring at(stages), acc(2);
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += step) {
+            const Tile c = tile_at(u, first, off, t);
+            const uint32_t idesc = idesc0 | ((c.rows + 15) / 16 * 2) << 17;
+            for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
+                const uint32_t end = min(kb + sect, kb1), from = kb;
+                ok = mbar_wait_warp(smem_u32(&ctl->tempty[acc.slot]), acc.pass ^ 1u, &ctl->abort);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + acc.slot * u.tmem_stride;
+                for (; kb < end; kb++, at.step()) {
+                    ok = mbar_wait_warp(full + at.slot * 8, at.pass, &ctl->abort);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d = tmem + acc.slot * u.tmem_stride;
-                    for (uint32_t from = kb; kb < end; kb++, at.step()) {
-                        if (aborted() || !mbar_wait(smem_u32(&ctl->xfull[at.slot]), at.pass) ||
-                            (INT4 && !mbar_wait(smem_u32(&ctl->afull[at.slot]), at.pass))) {
-                            ok = false;
-                            break;
-                        }
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = smem_u32(smem + (size_t)at.slot * stage_bytes);
-                        const uint64_t db = umma_desc(sa + A_PARTS * A_BYTES);
+                    const uint32_t sa = smem_u32(smem) + at.slot * stage_bytes;
+                    const uint64_t da = umma_desc(sa), db = umma_desc(sa + A_PARTS * A_BYTES);
+                    if (elect_one()) {
 #pragma unroll
-                        for (uint32_t a = 0; a < A_PARTS; a++) {
-                            const uint64_t da = umma_desc(sa + a * A_BYTES);
+                        for (uint32_t a = 0; a < A_PARTS; a++)
 #pragma unroll
                             for (uint32_t k = 0; k < BK / 16; k++)
-                                umma(d, da + 2 * k, db + 2 * k, idesc, kb != from || a || k);
-                        }
+                                umma(d, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k, idesc,
+                                     kb != from || a || k);
                         umma_commit(smem_u32(&ctl->empty[at.slot]));
                     }
-                    if (ok) umma_commit(smem_u32(&ctl->tfull[acc.slot]));
+                    __syncwarp();
                 }
+                if (ok && elect_one()) umma_commit(smem_u32(&ctl->tfull[acc.slot]));
+                __syncwarp();
             }
-            if (!ok) give_up();
-            umma_commit(smem_u32(&ctl->drain));  // completes once every MMA above has
         }
+        if (!ok) give_up();
+        if (elect_one()) umma_commit(smem_u32(&ctl->drain));  // completes once every MMA above has
+        __syncwarp();
     } else if (INT4 && warp == 3) {
-        if (lane == 0) {
-            const uint64_t per_expert = (uint64_t)nt * kbs;
-            Ring at(u.raw_stages);
-            bool ok = true;
-            for (uint32_t t = t0; ok && t < tiles; t += step) {
-                const Tile c = tile_at(u, first, off, t);
-                const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
-                                     (c.e * per_expert + (uint64_t)(c.n0 / 128) * kbs + kb0) * PK_BYTES;
-                for (uint32_t kb = kb0; kb < kb1; kb++, at.step(), src += PK_BYTES) {
-                    if (aborted() || !mbar_wait(smem_u32(&ctl->rempty[at.slot]), at.pass ^ 1u)) {
-                        ok = false;
-                        break;
-                    }
+        const uint64_t per_expert = (uint64_t)nt * kbs;
+        Ring at(u.raw_stages);
+        uint32_t issued = 0;
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += step) {
+            const Tile c = tile_at(u, first, off, t);
+            const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
+                                 (c.e * per_expert + (uint64_t)(c.n0 / 128) * kbs + kb0) * PK_BYTES;
+            for (uint32_t kb = kb0; kb < kb1; kb++, at.step(), src += PK_BYTES) {
+                ok = mbar_wait_warp(smem_u32(&ctl->rempty[at.slot]), at.pass ^ 1u, &ctl->abort);
+                if (!ok) break;
+                if (elect_one()) {
                     const uint32_t fb = smem_u32(&ctl->rfull[at.slot]);
                     mbar_expect_tx(fb, PK_BYTES);
                     bulk_load(smem_u32(raw + (size_t)at.slot * PK_BYTES), src, PK_BYTES, fb);
-                    *(volatile int *)&ctl->raw_issued = *(volatile int *)&ctl->raw_issued + 1;
                 }
+                __syncwarp();
+                issued++;
             }
-            if (!ok) give_up();
         }
+        if (lane == 0) ctl->raw_issued = (int)issued;
+        if (!ok) give_up();
     } else if (INT4 && warp >= 12) {
         // this group's K steps of all the CTA's tiles, one after another
         const uint32_t group = (warp - 12) >> 2, row = threadIdx.x & 127u;
@@ -864,7 +892,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         Ring in(u.raw_stages, group), to(stages, group);
         const uint32_t mine = row * 128 + ((row & 7u) << 4);  // chunk c of my row: ^ (c << 4)
         for (uint64_t it = group; it < steps; it += GROUPS, in.step(GROUPS), to.step(GROUPS)) {
-            if (aborted() || !mbar_wait(smem_u32(&ctl->rfull[in.slot]), in.pass)) {
+            if (!mbar_wait_warp(smem_u32(&ctl->rfull[in.slot]), in.pass, &ctl->abort)) {
                 give_up();
                 break;
             }
@@ -876,7 +904,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                 q[g] = *reinterpret_cast<const uint4 *>(src + (g * 128 + row) * 16);
                 sc[g] = *reinterpret_cast<const uint16_t *>(src + PK_NIB + (g * 128 + row) * 2);
             }
-            if (!mbar_wait(smem_u32(&ctl->empty[to.slot]), to.pass ^ 1u)) {
+            if (!mbar_wait_warp(smem_u32(&ctl->empty[to.slot]), to.pass ^ 1u, &ctl->abort)) {
                 give_up();
                 break;
             }
@@ -922,10 +950,9 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                     for (int j = 0; j < 16; j++) sum[i][j] = 0.0f;
             }
             for (uint32_t kb = kb0; kb < kb1; kb += sect, acc.step()) {
-                if (!mbar_wait(smem_u32(&ctl->tfull[acc.slot]), acc.pass) || aborted()) {
-                    ok = false;
-                    break;
-                }
+                ok = mbar_wait_warp(smem_u32(&ctl->tfull[acc.slot]), acc.pass, &ctl->abort);
+                if (!PRECISE) ok = set_agrees(set, ok);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ta = tmem + acc.slot * u.tmem_stride + ((q * 32) << 16);
                 if (PRECISE) {
@@ -960,6 +987,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[acc.slot]));
             }
+            if (PRECISE) ok = set_agrees(set, ok);
             if (PRECISE && ok) {
 #pragma unroll
                 for (int i = 0; i < (PRECISE ? CHUNKS : 1); i++) {
@@ -1013,15 +1041,17 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     __syncthreads();
     if (threadIdx.x == 0 && aborted()) {
         // the latest load into each slot (its phase completes only with the copy)
-        const int issued = *(volatile int *)&ctl->issued, got = *(volatile int *)&ctl->raw_issued;
+        const int issued = ctl->issued, got = ctl->raw_issued, go_on = 0;
         for (int it = max(0, issued - (int)stages); it < issued; it++)
-            if (!mbar_wait(smem_u32(&ctl->xfull[it % stages]), (uint32_t)(it / stages) & 1u)) give_up();
+            mbar_wait(smem_u32(&ctl->xfull[it % stages]), (uint32_t)(it / stages) & 1u, &go_on);
         for (int it = max(0, got - (int)u.raw_stages); it < got; it++)
-            if (!mbar_wait(smem_u32(&ctl->rfull[it % u.raw_stages]),
-                           (uint32_t)(it / u.raw_stages) & 1u))
-                give_up();
+            mbar_wait(smem_u32(&ctl->rfull[it % u.raw_stages]), (uint32_t)(it / u.raw_stages) & 1u,
+                      &go_on);
     }
-    if (threadIdx.x == 32 && !mbar_wait(smem_u32(&ctl->drain), 0)) give_up();
+    if (threadIdx.x == 32) {
+        const int go_on = 0;
+        if (!mbar_wait(smem_u32(&ctl->drain), 0, &go_on)) give_up();
+    }
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
