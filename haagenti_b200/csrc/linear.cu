@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -288,6 +289,11 @@ __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParam
 //   warps 12-23 INT4 only: three groups of 128 threads dequantise every third
 //               K step, a thread per weight row, into the 128B-swizzled A tile
 //
+// PAIR: where whole tiles of rows keep every SM busy, two CTAs share one tile of
+// 256 features (cta_group::2): each holds the weights of its 128 features and
+// half of the rows, so that a K step moves 32 KB instead of 48 KB from L2 to
+// each SM for the same MMAs.  The first CTA's MMA warp issues for both.
+//
 // With at least one tile per SM the kernel is persistent (grid = SMs) and the
 // accumulators are double-buffered, so a tile's epilogue runs under the next
 // tile's MMAs.  With fewer, the K range of a tile is split over a cluster of
@@ -345,11 +351,29 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Arrival on the barrier at the same place in CTA `rank` of the cluster.  What it
+// reports is in this SM (its A tile behind a proxy fence, its TMEM read behind a
+// tcgen05 fence) and is used there by the pair's MMA, so the release is at this
+// CTA's scope; one at cluster scope took over 1000 clocks a K step.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar),
+        "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+// Acquires at cluster scope: arrivals may come from the other CTA of a pair.
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -411,21 +435,38 @@ struct Ring {
         }
     }
 };
+// PAIR: the barrier may be the other CTA's.
+template <bool PAIR>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x,
                                        int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+            : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x,
                                        int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
                                           uint32_t bar) {
@@ -440,19 +481,61 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
            (2ull << 61);
 }
+template <bool PAIR>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
                                      uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
+// Arrives, once the MMAs issued before have completed, on the barrier at this
+// place: of both CTAs of a pair.
+template <bool PAIR>
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+            " [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+            : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t to, uint32_t cols) {
+    if (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to),
+                     "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to),
+                     "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
+    if (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols)
+                     : "memory");
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols)
+                     : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -483,10 +566,11 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t saddr, uint32_t rank) {
 struct Tile {
     uint32_t e, m0, rows, n0;
 };
+template <uint32_t FEATURES>
 __device__ __forceinline__ Tile tile_at(const UmmaParams &u, const uint32_t *first,
                                         const uint32_t *off, uint32_t t) {
     const LinParams &p = u.p;
-    const uint32_t nt = (p.N + 127) / 128;
+    const uint32_t nt = (p.N + FEATURES - 1) / FEATURES;
     Tile r;
     r.e = expert_of(first, p.E, t / nt);
     const uint32_t lo = off[r.e], hi = off[r.e + 1], m = hi - lo, mts = (m + u.bn - 1) / u.bn;
@@ -498,7 +582,7 @@ __device__ __forceinline__ Tile tile_at(const UmmaParams &u, const uint32_t *fir
     const uint32_t grp = q / (RASTER * nt), in = q - grp * RASTER * nt;
     const uint32_t width = min(RASTER, mts - grp * RASTER);
     const uint32_t mt = grp * RASTER + in % width;
-    r.n0 = in / width * 128;
+    r.n0 = in / width * FEATURES;
     r.m0 = lo + mt * per;
     r.rows = min(per, hi - r.m0);
     return r;
@@ -730,16 +814,17 @@ constexpr int umma_threads(bool int4) { return int4 ? 768 : 384; }
 // rows per tile at most: a thread of the epilogue keeps half of them as f32 sums where PRECISE
 __host__ __device__ constexpr uint32_t max_rows(bool int4, bool precise) { return precise ? (int4 ? 64 : 128) : 256; }
 
-template <bool INT4, bool BF, bool PRECISE>
+template <bool INT4, bool BF, bool PRECISE, bool PAIR>
 __global__ void __launch_bounds__(umma_threads(INT4), 1)
     linear_umma_kernel(const __grid_constant__ CUtensorMap tmX,
                        const __grid_constant__ CUtensorMap tmW, const __grid_constant__ UmmaParams u) {
     constexpr uint32_t A_PARTS = INT4 && PRECISE ? 2 : 1;
     constexpr uint32_t GROUPS = 3;  // of dequantising warps
+    constexpr uint32_t FEATURES = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const LinParams &p = u.p;
-    const uint32_t stages = u.stages, stage_bytes = A_PARTS * A_BYTES + u.bn * 128;
+    const uint32_t stages = u.stages, stage_bytes = A_PARTS * A_BYTES + u.bn / CTAS * 128;
     uint8_t *raw = smem + (size_t)stages * stage_bytes;
     uint8_t *epi = raw + (size_t)u.raw_stages * PK_BYTES;
     Ctl *ctl = reinterpret_cast<Ctl *>(epi + EPI_BYTES);
@@ -749,7 +834,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < stages; s++) {
             mbar_init(smem_u32(&ctl->xfull[s]), 1);
-            mbar_init(smem_u32(&ctl->afull[s]), 4);
+            mbar_init(smem_u32(&ctl->afull[s]), 4 * CTAS);
             mbar_init(smem_u32(&ctl->empty[s]), 1);
         }
         for (uint32_t s = 0; s < u.raw_stages; s++) {
@@ -758,7 +843,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(smem_u32(&ctl->tfull[b]), 1);
-            mbar_init(smem_u32(&ctl->tempty[b]), 8);
+            mbar_init(smem_u32(&ctl->tempty[b]), 8 * CTAS);
         }
         mbar_init(smem_u32(&ctl->drain), 1);
         ctl->abort = 0;
@@ -768,15 +853,12 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(&ctl->tmem_base)),
-                     "r"(u.tmem_cols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tmem_alloc<PAIR>(smem_u32(&ctl->tmem_base), u.tmem_cols);
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
     if (warp == 2) scan_groups(p, u.bn, first, off);
     __syncthreads();
+    if (PAIR) cluster_barrier();  // the other CTA's barriers are set up too
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = ctl->tmem_base;
     const auto aborted = [&] { return *(volatile int *)&ctl->abort != 0; };
@@ -785,10 +867,10 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         atomicExch(&ctl->abort, 1);
     };
 
-    const uint32_t nt = (p.N + 127) / 128;
-    const uint32_t tiles = first[p.E] * nt;
-    const uint32_t rank = blockIdx.x % u.split;  // clusters are consecutive CTAs
-    const uint32_t t0 = blockIdx.x / u.split, step = gridDim.x / u.split;
+    const uint32_t tiles = first[p.E] * ((p.N + FEATURES - 1) / FEATURES);
+    // clusters are consecutive CTAs: the parts of a K range, or a pair
+    const uint32_t rank = blockIdx.x % u.split, side = PAIR ? blockIdx.x & 1u : 0u;
+    const uint32_t t0 = blockIdx.x / (PAIR ? 2 : u.split), step = gridDim.x / (PAIR ? 2 : u.split);
     const uint32_t kbs = (p.K + BK - 1) / BK;
     const uint32_t kb0 = (uint32_t)((uint64_t)kbs * rank / u.split);
     const uint32_t kb1 = (uint32_t)((uint64_t)kbs * (rank + 1) / u.split);
@@ -801,20 +883,26 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         uint32_t issued = 0;
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at(u, first, off, t);
-            const uint32_t boxes = (c.rows + u.xbox - 1) / u.xbox;
-            const uint32_t bytes = boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES);
+            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            // each CTA of a pair holds its 128 features and half of the tile's rows,
+            // and both copies complete on the leader's barrier
+            const uint32_t held = (c.rows + 15) / 16 * 16 / CTAS;
+            const uint32_t boxes = (held + u.xbox - 1) / u.xbox;
+            const uint32_t bytes = (boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES)) * CTAS;
+            const int m0 = (int)(c.m0 + side * held), n0 = (int)(c.n0 + side * 128);
             for (uint32_t kb = kb0; kb < kb1; kb++, at.step()) {
                 ok = mbar_wait_warp(smem_u32(&ctl->empty[at.slot]), at.pass ^ 1u, &ctl->abort);
                 if (!ok) break;
                 if (elect_one()) {
                     const uint32_t sa = smem_u32(smem + (size_t)at.slot * stage_bytes);
-                    const uint32_t sb = sa + A_PARTS * A_BYTES, fb = smem_u32(&ctl->xfull[at.slot]);
-                    mbar_expect_tx(fb, bytes);
-                    if (!INT4) tma_3d(sa, &tmW, fb, (int)(kb * BK), (int)c.n0, (int)c.e);
+                    const uint32_t sb = sa + A_PARTS * A_BYTES;
+                    uint32_t fb = smem_u32(&ctl->xfull[at.slot]);
+                    if (side == 0) mbar_expect_tx(fb, bytes);
+                    if (PAIR) fb = map_to(fb, 0);
+                    if (!INT4) tma_3d<PAIR>(sa, &tmW, fb, (int)(kb * BK), n0, (int)c.e);
                     for (uint32_t b = 0; b < boxes; b++)
-                        tma_2d(sb + b * u.xbox * 128, &tmX, fb, (int)(kb * BK),
-                               (int)(c.m0 + b * u.xbox));
+                        tma_2d<PAIR>(sb + b * u.xbox * 128, &tmX, fb, (int)(kb * BK),
+                                     m0 + (int)(b * u.xbox));
                 }
                 __syncwarp();
                 issued++;
@@ -823,14 +911,15 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         if (lane == 0) ctl->issued = (int)issued;
         if (!ok) give_up();
     } else if (warp == 1) {
-        // D = F32, A = B = x's type, both K-major, M = 128; N follows the tile
-        const uint32_t idesc0 = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);
+        // D = F32, A = B = x's type, both K-major, M = FEATURES; N follows the tile
+        const uint32_t idesc0 =
+            (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((FEATURES / 16) << 24);
         // INT4: half of the lanes wait for the x tile, half for the weights
         const uint32_t full = smem_u32(INT4 && lane >= 16 ? ctl->afull : ctl->xfull);
         Ring at(stages), acc(2);
         bool ok = true;
-        for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at(u, first, off, t);
+        for (uint32_t t = t0; side == 0 && ok && t < tiles; t += step) {
+            const Tile c = tile_at<FEATURES>(u, first, off, t);
             const uint32_t idesc = idesc0 | ((c.rows + 15) / 16 * 2) << 17;
             for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
                 const uint32_t end = min(kb + sect, kb1), from = kb;
@@ -849,28 +938,30 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                         for (uint32_t a = 0; a < A_PARTS; a++)
 #pragma unroll
                             for (uint32_t k = 0; k < BK / 16; k++)
-                                umma(d, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k, idesc,
-                                     kb != from || a || k);
-                        umma_commit(smem_u32(&ctl->empty[at.slot]));
+                                umma<PAIR>(d, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k, idesc,
+                                           kb != from || a || k);
+                        umma_commit<PAIR>(smem_u32(&ctl->empty[at.slot]));
                     }
                     __syncwarp();
                 }
-                if (ok && elect_one()) umma_commit(smem_u32(&ctl->tfull[acc.slot]));
+                if (ok && elect_one()) umma_commit<PAIR>(smem_u32(&ctl->tfull[acc.slot]));
                 __syncwarp();
             }
         }
         if (!ok) give_up();
-        if (elect_one()) umma_commit(smem_u32(&ctl->drain));  // completes once every MMA above has
+        // completes once every MMA above has, in both CTAs
+        if (side == 0 && elect_one()) umma_commit<PAIR>(smem_u32(&ctl->drain));
         __syncwarp();
     } else if (INT4 && warp == 3) {
-        const uint64_t per_expert = (uint64_t)nt * kbs;
+        const uint32_t nt = (p.N + 127) / 128;
         Ring at(u.raw_stages);
         uint32_t issued = 0;
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at(u, first, off, t);
-            const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
-                                 (c.e * per_expert + (uint64_t)(c.n0 / 128) * kbs + kb0) * PK_BYTES;
+            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            // a pair's second half may lie past the last features: any block will do there
+            const uint64_t block = (uint64_t)c.e * nt + min(c.n0 / 128 + side, nt - 1);
+            const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) + (block * kbs + kb0) * PK_BYTES;
             for (uint32_t kb = kb0; kb < kb1; kb++, at.step(), src += PK_BYTES) {
                 ok = mbar_wait_warp(smem_u32(&ctl->rempty[at.slot]), at.pass ^ 1u, &ctl->abort);
                 if (!ok) break;
@@ -926,7 +1017,8 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(smem_u32(&ctl->afull[to.slot]));
+                if (PAIR) mbar_arrive_at(smem_u32(&ctl->afull[to.slot]), 0);
+                else mbar_arrive(smem_u32(&ctl->afull[to.slot]));
                 mbar_arrive(smem_u32(&ctl->rempty[in.slot]));
             }
         }
@@ -938,8 +1030,8 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         Ring acc(2);
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at(u, first, off, t);
-            const uint32_t n = c.n0 + id % 16 * 8;
+            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            const uint32_t n = c.n0 + side * 128 + id % 16 * 8;
             float bias[8];
             if (u.split == 1) load_bias8<BF>(p, c.e, n, bias);
             float sum[PRECISE ? CHUNKS : 1][16];
@@ -985,7 +1077,10 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->tempty[acc.slot]));
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_at(smem_u32(&ctl->tempty[acc.slot]), 0);
+                    else mbar_arrive(smem_u32(&ctl->tempty[acc.slot]));
+                }
             }
             if (PRECISE) ok = set_agrees(set, ok);
             if (PRECISE && ok) {
@@ -1005,14 +1100,14 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         if (!ok) give_up();
     }
 
-    if (u.split > 1) {
+    if (!PAIR && u.split > 1) {
         // one tile per cluster: each CTA finishes its share of the tile's rows,
         // adding the CTAs' parts in rank order.  Both barriers are reached by
         // every thread of every CTA on every path.
         __syncwarp();
         cluster_barrier();
         if (t0 < tiles && !aborted()) {
-            const Tile c = tile_at(u, first, off, t0);
+            const Tile c = tile_at<FEATURES>(u, first, off, t0);
             const uint32_t j0 = c.rows * rank / u.split, j1 = c.rows * (rank + 1) / u.split;
             const uint32_t f = threadIdx.x % 16 * 8, n = c.n0 + f, base = smem_u32(smem);
             if (n < p.N) {
@@ -1040,9 +1135,10 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     // ---- teardown: nothing of this CTA may be in flight when it ends --------------
     __syncthreads();
     if (threadIdx.x == 0 && aborted()) {
-        // the latest load into each slot (its phase completes only with the copy)
+        // the latest load into each slot (its phase completes only with the copy; a
+        // pair's x and dense copies complete on the leader's barriers)
         const int issued = ctl->issued, got = ctl->raw_issued, go_on = 0;
-        for (int it = max(0, issued - (int)stages); it < issued; it++)
+        for (int it = max(0, issued - (int)stages); side == 0 && it < issued; it++)
             mbar_wait(smem_u32(&ctl->xfull[it % stages]), (uint32_t)(it / stages) & 1u, &go_on);
         for (int it = max(0, got - (int)u.raw_stages); it < got; it++)
             mbar_wait(smem_u32(&ctl->rfull[it % u.raw_stages]), (uint32_t)(it / u.raw_stages) & 1u,
@@ -1053,11 +1149,10 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         if (!mbar_wait(smem_u32(&ctl->drain), 0, &go_on)) give_up();
     }
     __syncthreads();
+    if (PAIR) cluster_barrier();  // neither CTA's memory is in use any more
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                     "r"(u.tmem_cols)
-                     : "memory");
+        tmem_free<PAIR>(tmem, u.tmem_cols);
     }
 }
 
@@ -1206,10 +1301,10 @@ bool tma_rows(const void *base, uint64_t rows, uint64_t ld, uint64_t K) {
 
 inline uint32_t round_to(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
 
-template <bool INT4, bool BF, bool PRECISE>
+template <bool INT4, bool BF, bool PRECISE, bool PAIR>
 cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const UmmaParams &u,
                         uint32_t grid, uint32_t smem, cudaStream_t s) {
-    const auto kernel = linear_umma_kernel<INT4, BF, PRECISE>;
+    const auto kernel = linear_umma_kernel<INT4, BF, PRECISE, PAIR>;
     // once per device (64 of them remembered); twice by two threads does no harm
     static std::atomic<uint64_t> set{0};
     int dev = 0;
@@ -1227,57 +1322,70 @@ cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const Umma
     c.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = u.split;
+    attr[0].val.clusterDim.x = PAIR ? 2 : u.split;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     c.attrs = attr;
     c.numAttrs = 1;
     return cudaLaunchKernelEx(&c, kernel, tx, tw, u);
 }
 
-// Tile height, split and ring depths of a call on the tensor-core kernel.
+// Rows per tile of M rows by nt feature tiles on `units` SMs or pairs of them:
+// the height whose waves of tiles take the least time, waves x (rows + what a
+// tile's K step costs beside its rows).
+uint32_t tile_rows(uint32_t M, uint32_t nt, uint32_t units, uint32_t cap) {
+    if (M <= cap) return round_to(M, 16);
+    uint32_t rows = cap;
+    uint64_t best = ~0ull;
+    for (uint32_t bn = cap; bn >= cap / 2; bn -= 16) {
+        const uint64_t mts = (M + bn - 1) / bn;
+        const uint32_t per = round_to((uint32_t)((M + mts - 1) / mts), 16);
+        const uint64_t cost = (mts * nt + units - 1) / units * (per + 32);
+        if (cost < best) {
+            best = cost;
+            rows = bn;
+        }
+    }
+    return rows;
+}
+
+// Pair or single, tile height, split and ring depths of a call on the
+// tensor-core kernel.
 cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaStream_t s) {
     const bool precise = p.odt == HCT_B200_F32;
     const uint32_t sms = (uint32_t)sm_count(), cap = max_rows(int4, precise);
-    const uint32_t nt = (p.N + 127) / 128, kbs = (p.K + BK - 1) / BK;
+    const uint32_t kbs = (p.K + BK - 1) / BK;
+    const uint32_t active = std::min(p.E, p.M), per_expert = p.M / active;
     UmmaParams u{};
     u.p = p;
+    u.split = 1;
+    // pairs where tiles of 256 features and full height keep every pair busy
+    const bool pair = !precise && per_expert >= 192 &&
+                      (uint64_t)((p.N + 255) / 256) * (p.M / 256) * 2 >= sms;
+    const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128, units = pair ? sms / 2 : sms;
     uint64_t row_tiles;  // at most
-    if (!grouped) {
-        if (p.M <= cap) {
-            u.bn = round_to(p.M, 16);
-        } else {
-            // the height whose waves of tiles take the least time: waves x (rows +
-            // what a tile costs beside its rows)
-            uint64_t best = ~0ull;
-            for (uint32_t bn = cap; bn >= cap / 2; bn -= 16) {
-                const uint64_t mts = (p.M + bn - 1) / bn;
-                const uint32_t per = round_to((uint32_t)((p.M + mts - 1) / mts), 16);
-                const uint64_t cost = (mts * nt + sms - 1) / sms * (per + 16);
-                if (cost < best) {
-                    best = cost;
-                    u.bn = bn;
-                }
-            }
-        }
-        u.xbox = u.bn;
-        row_tiles = (p.M + u.bn - 1) / u.bn;
-    } else {
-        const uint32_t active = std::min(p.E, p.M);
-        u.bn = std::min(cap, p.M / active <= 64 ? 128u : 256u);
+    if (grouped) {
+        u.bn = std::min(cap, per_expert <= 64 ? 128u : 256u);
         u.xbox = 32;
         row_tiles = p.M / u.bn + active;
+    } else {
+        u.bn = tile_rows(p.M, nt, units, cap);
+        u.xbox = pair ? u.bn / 2 : u.bn;
+        row_tiles = (p.M + u.bn - 1) / u.bn;
     }
     const uint64_t tiles = row_tiles * nt;
     if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
-    // fewer tiles than half the SMs: the K range is split over a cluster
-    u.split = 1;
-    if (tiles * 2 <= sms) u.split = std::min<uint32_t>({8u, (uint32_t)(sms / tiles), kbs});
-    const uint32_t grid = u.split > 1 ? (uint32_t)tiles * u.split
-                                      : (uint32_t)std::min<uint64_t>(tiles, sms);
+    uint32_t grid;
+    if (pair) {
+        grid = 2 * (uint32_t)std::min<uint64_t>(tiles, units);
+    } else {
+        // fewer tiles than half the SMs: the K range is split over a cluster
+        if (tiles * 2 <= sms) u.split = std::min<uint32_t>({8u, (uint32_t)(sms / tiles), kbs});
+        grid = u.split > 1 ? (uint32_t)tiles * u.split : (uint32_t)std::min<uint64_t>(tiles, sms);
+    }
     u.tmem_stride = round_to(u.bn, 32);
     u.tmem_cols = 64;
     while (u.tmem_cols < 2 * u.tmem_stride) u.tmem_cols *= 2;
-    const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn * 128;
+    const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn / (pair ? 2 : 1) * 128;
     u.raw_stages = int4 ? 10 : 0;
     const uint32_t fixed =
         1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) + (p.E + 1) * 8;
@@ -1294,16 +1402,16 @@ cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaS
         if (!operand_map(&tw, bf, p.w, p.K, p.N, ld, p.E, p.E == 1 ? ld * p.N : p.w_stride, 128))
             return cudaErrorInvalidValue;
     }
-    if (int4) {
-        if (bf) return precise ? launch_umma<true, true, true>(tx, tw, u, grid, smem, s)
-                               : launch_umma<true, true, false>(tx, tw, u, grid, smem, s);
-        return precise ? launch_umma<true, false, true>(tx, tw, u, grid, smem, s)
-                       : launch_umma<true, false, false>(tx, tw, u, grid, smem, s);
-    }
-    if (bf) return precise ? launch_umma<false, true, true>(tx, tw, u, grid, smem, s)
-                           : launch_umma<false, true, false>(tx, tw, u, grid, smem, s);
-    return precise ? launch_umma<false, false, true>(tx, tw, u, grid, smem, s)
-                   : launch_umma<false, false, false>(tx, tw, u, grid, smem, s);
+    const auto launch = [&](auto is_int4, auto is_bf) {
+        constexpr bool I = decltype(is_int4)::value, B = decltype(is_bf)::value;
+        if (precise) return launch_umma<I, B, true, false>(tx, tw, u, grid, smem, s);
+        if (pair) return launch_umma<I, B, false, true>(tx, tw, u, grid, smem, s);
+        return launch_umma<I, B, false, false>(tx, tw, u, grid, smem, s);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (int4) return bf ? launch(yes, yes) : launch(yes, no);
+    return bf ? launch(no, yes) : launch(no, no);
 }
 
 int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {

@@ -115,7 +115,9 @@ SHAPES = [(1, 1, 32), (1, 8, 64), (1, 128, 4096), (1, 1000, 1024), (2, 130, 96),
           (5, 384, 672), (8, 128, 8192), (9, 640, 512), (15, 100, 160), (16, 256, 256), (17, 129, 320),
           (31, 513, 1056), (33, 128, 64), (64, 1024, 1024), (65, 200, 128), (100, 777, 992),
           (127, 128, 448), (128, 128, 128), (129, 384, 512), (200, 1000, 608), (255, 130, 96),
-          (256, 256, 1024), (257, 300, 640), (300, 2048, 256), (513, 640, 800), (1000, 1153, 320)]
+          (256, 256, 1024), (257, 300, 640), (300, 2048, 256), (513, 640, 800), (1000, 1153, 320),
+          # enough whole tiles for pairs of CTAs: a second half past the last feature, odd heights
+          (300, 19000, 96), (513, 9728, 160), (1030, 4900, 320), (700, 9600, 1056)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -194,7 +196,8 @@ def sorted_sizes(kind, m, e, seed):
 
 @pytest.mark.parametrize("m,e,n,k", [(1, 1, 32, 32), (1, 8, 256, 512), (8, 8, 1000, 1024),
                                      (8, 64, 64, 96), (40, 3, 384, 2048), (96, 16, 130, 160),
-                                     (257, 5, 200, 64), (1000, 7, 257, 320), (1500, 40, 128, 256)])
+                                     (257, 5, 200, 64), (1000, 7, 257, 320), (1500, 40, 128, 256),
+                                     (1500, 3, 7710, 160), (2100, 7, 2400, 320)])
 @pytest.mark.parametrize("kind", ["even", "one", "ragged"])
 @pytest.mark.parametrize("form,dt,out", [("int4", "bf16", "bf16"), ("int4", "f16", "f32"),
                                          ("dense", "bf16", "f32"), ("dense", "f16", "f16")])
