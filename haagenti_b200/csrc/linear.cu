@@ -481,6 +481,10 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
            (2ull << 61);
 }
+// A value that is the same in every lane, in a form that lets the compiler keep
+// it (and the addresses and descriptors made of it) in uniform registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 template <bool PAIR>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
                                      uint32_t accumulate) {
@@ -829,7 +833,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     uint8_t *epi = raw + (size_t)u.raw_stages * PK_BYTES;
     Ctl *ctl = reinterpret_cast<Ctl *>(epi + EPI_BYTES);
     uint32_t *first = reinterpret_cast<uint32_t *>(ctl + 1), *off = first + p.E + 1;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < stages; s++) {
@@ -860,14 +864,14 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     __syncthreads();
     if (PAIR) cluster_barrier();  // the other CTA's barriers are set up too
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = uniform(ctl->tmem_base);
     const auto aborted = [&] { return *(volatile int *)&ctl->abort != 0; };
     const auto give_up = [&] {
         atomicExch(&g_linear_status, HCT_B200_ERR_TIMEOUT);
         atomicExch(&ctl->abort, 1);
     };
 
-    const uint32_t tiles = first[p.E] * ((p.N + FEATURES - 1) / FEATURES);
+    const uint32_t tiles = uniform(first[p.E]) * ((p.N + FEATURES - 1) / FEATURES);
     // clusters are consecutive CTAs: the parts of a K range, or a pair
     const uint32_t rank = blockIdx.x % u.split, side = PAIR ? blockIdx.x & 1u : 0u;
     const uint32_t t0 = blockIdx.x / (PAIR ? 2 : u.split), step = gridDim.x / (PAIR ? 2 : u.split);
@@ -920,7 +924,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         bool ok = true;
         for (uint32_t t = t0; side == 0 && ok && t < tiles; t += step) {
             const Tile c = tile_at<FEATURES>(u, first, off, t);
-            const uint32_t idesc = idesc0 | ((c.rows + 15) / 16 * 2) << 17;
+            const uint32_t idesc = uniform(idesc0 | ((c.rows + 15) / 16 * 2) << 17);
             for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
                 const uint32_t end = min(kb + sect, kb1), from = kb;
                 ok = mbar_wait_warp(smem_u32(&ctl->tempty[acc.slot]), acc.pass ^ 1u, &ctl->abort);
@@ -1117,11 +1121,21 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                     Operands o;
                     load_operands<PRECISE ? HCT_B200_F32 : HCT_B200_F16>(p, c.m0 + j, n, o);
                     float z[8] = {};
-                    for (uint32_t r = 0; r < u.split; r++) {
-                        const float4 a = ld_cluster(base + (j * 128 + f) * 4, r);
-                        const float4 b = ld_cluster(base + (j * 128 + f + 4) * 4, r);
-                        z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
-                        z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
+#pragma unroll
+                    for (uint32_t r0 = 0; r0 < 8; r0 += 4) {  // four parts in flight
+                        float4 a[4], b[4];
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; i++)
+                            if (r0 + i < u.split) {
+                                a[i] = ld_cluster(base + (j * 128 + f) * 4, r0 + i);
+                                b[i] = ld_cluster(base + (j * 128 + f + 4) * 4, r0 + i);
+                            }
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; i++)
+                            if (r0 + i < u.split) {
+                                z[0] += a[i].x, z[1] += a[i].y, z[2] += a[i].z, z[3] += a[i].w;
+                                z[4] += b[i].x, z[5] += b[i].y, z[6] += b[i].z, z[7] += b[i].w;
+                            }
                     }
 #pragma unroll
                     for (int i = 0; i < 8; i++) z[i] += bias[i];
