@@ -26,8 +26,11 @@ constexpr uint64_t DIM_LIMIT = 1ull << 31;
 // A packed matrix is a sequence of blocks [ceil(rows / 128)][ceil(cols / 64)],
 // each 128 rows x 64 columns (two scale blocks per row), 4608 contiguous
 // bytes, so that one bulk copy brings everything a K step of a tile needs:
-//   nibbles  [2 scale blocks][128 rows][16 bytes]   (16 B per thread, conflict-free)
-//   scales   [2 scale blocks][128 rows] f16
+//   nibbles  [2 scale blocks][128 rows][16 bytes]
+//   scales   [2 scale blocks][8][16] f16, that of row r at [r % 8][r / 8]
+// A row's 16 bytes are what a dequantising thread takes, and the 4-byte words
+// of 8 consecutive rows are what a warp's mma fragment takes (the lane of row
+// r % 8 needs the scales of rows r % 8 + 8 i: 32 bytes in a row).
 // Each 32-bit word holds the 8 values k = 8 c .. 8 c + 7 of its scale block,
 // value 2 j in bits 4 j .. 4 j + 3 and value 2 j + 1 in bits 16 + 4 j .., so
 // that (word >> 4 j) & 0x000f000f is the pair (2 j, 2 j + 1) in two 16-bit
@@ -37,6 +40,7 @@ constexpr uint32_t PK_NIB = PK_ROWS * PK_COLS / 2;       // 4096
 constexpr uint32_t PK_BYTES = PK_NIB + PK_ROWS * 2 * 2;  // 4608
 
 __host__ __device__ inline uint64_t pk_kblocks(uint64_t cols) { return (cols + PK_COLS - 1) / PK_COLS; }
+__host__ __device__ inline uint32_t pk_scale_at(uint32_t row) { return row % 8 * 16 + row / 8; }
 inline uint64_t pk_bytes(uint64_t rows, uint64_t cols) {
     return (rows + PK_ROWS - 1) / PK_ROWS * pk_kblocks(cols) * PK_BYTES;
 }
@@ -72,7 +76,7 @@ __global__ void int4_weight_pack_kernel(const uint8_t *__restrict__ data, uint64
         }
         uint8_t *o = out + blk * PK_BYTES;
         *reinterpret_cast<uint4 *>(o + in * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint16_t *>(o + PK_NIB + in * 2) = scale;
+        *reinterpret_cast<uint16_t *>(o + PK_NIB + (g * PK_ROWS + pk_scale_at(r)) * 2) = scale;
     }
 }
 
@@ -237,7 +241,8 @@ __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParam
                         const uint32_t word = *reinterpret_cast<const uint32_t *>(b + in * 16 + c * 4);
                         const uint32_t q = word >> (4 * (k % 8 / 2) + 16 * (k % 2)) & 15u;
                         v = (float)((int)q - 8) *
-                            h2f(*reinterpret_cast<const uint16_t *>(b + PK_NIB + in * 2));
+                            h2f(*reinterpret_cast<const uint16_t *>(
+                                b + PK_NIB + (k / 32 % 2 * PK_ROWS + pk_scale_at(n % PK_ROWS)) * 2));
                     } else {
                         v = from16<BF>(reinterpret_cast<const uint16_t *>(
                             p.w)[(uint64_t)e * p.w_stride + (uint64_t)n * p.ldw + k]);
@@ -997,7 +1002,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 q[g] = *reinterpret_cast<const uint4 *>(src + (g * 128 + row) * 16);
-                sc[g] = *reinterpret_cast<const uint16_t *>(src + PK_NIB + (g * 128 + row) * 2);
+                sc[g] = *reinterpret_cast<const uint16_t *>(src + PK_NIB + (g * 128 + pk_scale_at(row)) * 2);
             }
             if (!mbar_wait_warp(smem_u32(&ctl->empty[to.slot]), to.pass ^ 1u, &ctl->abort)) {
                 give_up();
@@ -1170,6 +1175,269 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     }
 }
 
+// ---- INT4 stream kernel: a few rows of x -----------------------------------------
+//
+// Up to 8 NT rows against 128 features: nothing but the stream of packed
+// weights costs, and one kernel step per 4.5 bits has to keep up with HBM.
+// Each warp takes every WARPS-th K block of 64 of the CTA's range, brought
+// into its own two-slot ring by bulk copies (no other warp waits for it), and
+// feeds mma.sync m16n8k16 straight from registers: the nibbles less 8 are
+// exact in x's type, so a scale block's products are exact integers times x,
+// summed in f32, and the block's scale multiplies that sum in f32.  No weight
+// is rounded, for any output type.  A lane's A fragment is 8 consecutive k of
+// a row and its B fragment the same 8 of a row of x: the order of k inside a
+// scale block does not matter to the sum.
+//
+// The warps' sums meet in shared memory; where tiles are few, the K range is
+// also split over a cluster, whose CTAs push their sums to the CTA that
+// finishes the row (added in rank order).
+constexpr int ST_WARPS = 8, ST_THREADS = ST_WARPS * 32, ST_SLOTS = 2;
+
+struct StreamParams {
+    LinParams p;
+    uint32_t split;
+    int vec_x;  // rows of x start on 16-byte boundaries
+};
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The pairs of a word as nibble - 8 in x's type (see dequant8).
+template <bool BF>
+__device__ __forceinline__ void nibbles8(uint32_t w, uint32_t (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (BF) {
+            uint32_t b = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+            v[j] = bits_of(__hsub2(*reinterpret_cast<__nv_bfloat162 *>(&b), __float2bfloat162_rn(136.0f)));
+        } else {
+            uint32_t b = (j & 1 ? (w >> (8 * (j / 2))) & 0x00f000f0u
+                                : (w >> (8 * (j / 2))) & 0x000f000fu) | 0x64006400u;
+            const __half2 m = *reinterpret_cast<__half2 *>(&b);
+            v[j] = bits_of(j & 1 ? __hfma2(m, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
+                                 : __hsub2(m, __float2half2_rn(1032.0f)));
+        }
+    }
+}
+
+// 8 values k .. k + 7 of row m of x, zero past the row's end and past `hi`.
+__device__ __forceinline__ uint4 load_x8(const StreamParams &q, uint32_t m, uint32_t hi, uint32_t k) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (m >= hi || k >= q.p.K) return v;  // K is a multiple of 32: 8 values or none
+    const uint16_t *s = reinterpret_cast<const uint16_t *>(q.p.x) + (uint64_t)m * q.p.ldx + k;
+    if (q.vec_x) return *reinterpret_cast<const uint4 *>(s);
+    v.x = s[0] | (uint32_t)s[1] << 16;
+    v.y = s[2] | (uint32_t)s[3] << 16;
+    v.z = s[4] | (uint32_t)s[5] << 16;
+    v.w = s[6] | (uint32_t)s[7] << 16;
+    return v;
+}
+
+template <bool BF, int NT>
+__global__ void __launch_bounds__(ST_THREADS, 2)
+    linear_int4_stream_kernel(const __grid_constant__ StreamParams q) {
+    constexpr uint32_t ROWS = 8 * NT;
+    extern __shared__ __align__(128) uint8_t st_smem[];
+    const LinParams &p = q.p;
+    uint8_t *ring = st_smem;                                                   // [warp][slot]
+    float *recv = reinterpret_cast<float *>(ring + ST_WARPS * ST_SLOTS * PK_BYTES);  // [ROWS][128]
+    uint64_t *full = reinterpret_cast<uint64_t *>(recv + ROWS * 128);           // [warp][slot]
+    uint32_t *first = reinterpret_cast<uint32_t *>(full + ST_WARPS * ST_SLOTS), *off = first + p.E + 1;
+    int *abort = reinterpret_cast<int *>(off + p.E + 1);
+    const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
+    if (threadIdx.x < ST_WARPS * ST_SLOTS) mbar_init(smem_u32(&full[threadIdx.x]), 1);
+    if (threadIdx.x == 0) *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (warp == 1) scan_groups(p, ROWS, first, off);
+    __syncthreads();
+    // the cluster's CTAs are all running before any of them writes to another
+    if (q.split > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+
+    const uint32_t nt = (p.N + 127) / 128, kbs = (uint32_t)pk_kblocks(p.K);
+    const uint32_t rank = blockIdx.x % q.split, t = blockIdx.x / q.split;
+    const bool work = t < first[p.E] * nt;  // of the whole cluster alike
+    uint32_t e = 0, m0 = 0, hi = 0, n0 = 0;
+    float acc[8][NT][4];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int c = 0; c < NT; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[i][c][j] = 0.0f;
+    bool ok = true;
+    if (work) {
+        e = expert_of(first, p.E, t / nt);
+        hi = off[e + 1];
+        m0 = off[e] + (t / nt - first[e]) * ROWS;
+        n0 = t % nt * 128;
+        const uint32_t kb0 = (uint32_t)((uint64_t)kbs * rank / q.split);
+        const uint32_t kb1 = (uint32_t)((uint64_t)kbs * (rank + 1) / q.split);
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
+                             ((uint64_t)e * nt + n0 / 128) * kbs * PK_BYTES;
+        uint8_t *mine = ring + warp * ST_SLOTS * PK_BYTES;
+        const auto fetch = [&](uint32_t kb, uint32_t slot) {
+            if (kb < kb1 && elect_one()) {
+                const uint32_t bar = smem_u32(&full[warp * ST_SLOTS + slot]);
+                mbar_expect_tx(bar, PK_BYTES);
+                bulk_load(smem_u32(mine + slot * PK_BYTES), src + (uint64_t)kb * PK_BYTES, PK_BYTES, bar);
+            }
+            __syncwarp();
+        };
+        const uint32_t gid = lane / 4, tig = lane % 4;
+        uint4 x[2][NT];
+        const auto fetch_x = [&](uint32_t kb) {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int c = 0; c < NT; c++)
+                    x[g][c] = load_x8(q, m0 + 8 * c + gid, kb < kb1 ? hi : 0, kb * 64 + g * 32 + tig * 8);
+        };
+        uint32_t kb = kb0 + warp;
+#pragma unroll
+        for (uint32_t s = 0; s < ST_SLOTS; s++) fetch(kb + s * ST_WARPS, s);
+        fetch_x(kb);
+        uint32_t slot = 0, pass = 0;
+        for (; kb < kb1; kb += ST_WARPS) {
+            uint4 b[2][NT];
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int c = 0; c < NT; c++) b[g][c] = x[g][c];
+            fetch_x(kb + ST_WARPS);
+            if (!mbar_wait_warp(smem_u32(&full[warp * ST_SLOTS + slot]), pass, abort)) {
+                ok = false;
+                break;
+            }
+            const uint8_t *blk = mine + slot * PK_BYTES;
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const uint32_t *nib = reinterpret_cast<const uint32_t *>(blk) + (g * 128 + gid) * 4 + tig;
+                const uint4 *sc = reinterpret_cast<const uint4 *>(blk + PK_NIB + (g * 128 + gid * 16) * 2);
+                const uint4 s0 = sc[0], s1 = sc[1];
+                const uint32_t s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {  // rows 16 i + gid and 16 i + 8 + gid
+                    uint32_t lo[4], up[4];
+                    nibbles8<BF>(nib[16 * i * 4], lo);
+                    nibbles8<BF>(nib[(16 * i + 8) * 4], up);
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&s[i]));
+#pragma unroll
+                    for (int c = 0; c < NT; c++) {
+                        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma16816<BF>(d, lo[0], up[0], lo[1], up[1], b[g][c].x, b[g][c].y);
+                        mma16816<BF>(d, lo[2], up[2], lo[3], up[3], b[g][c].z, b[g][c].w);
+                        acc[i][c][0] = fmaf(f.x, d[0], acc[i][c][0]);
+                        acc[i][c][1] = fmaf(f.x, d[1], acc[i][c][1]);
+                        acc[i][c][2] = fmaf(f.y, d[2], acc[i][c][2]);
+                        acc[i][c][3] = fmaf(f.y, d[3], acc[i][c][3]);
+                    }
+                }
+            }
+            __syncwarp();
+            fetch(kb + ST_SLOTS * ST_WARPS, slot);
+            if (++slot == ST_SLOTS) {
+                slot = 0;
+                pass ^= 1u;
+            }
+        }
+        if (!ok) {
+            // the copies in flight end before the CTA does (bounded)
+            atomicExch(&g_linear_status, HCT_B200_ERR_TIMEOUT);
+            const int go_on = 0;
+            for (uint32_t s = 0; s < ST_SLOTS; s++)
+                if (kb + s * ST_WARPS < kb1)
+                    mbar_wait(smem_u32(&full[warp * ST_SLOTS + (slot + s) % ST_SLOTS]),
+                              pass ^ (slot + s >= ST_SLOTS), &go_on);
+        }
+        // my sums, [row of x][128 features], over my ring (its copies are done)
+        __syncwarp();
+        float *part = reinterpret_cast<float *>(mine);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int c = 0; c < NT; c++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    part[(8 * c + 2 * tig + (j & 1)) * 128 + 16 * i + 8 * (j >> 1) + gid] = acc[i][c][j];
+    }
+    __syncthreads();
+    // a thread per row and 8 features: the warps' sums in warp order
+    const uint32_t rows = work ? min(ROWS, hi - m0) : 0;
+    const uint32_t row = threadIdx.x / 16, f = threadIdx.x % 16 * 8, n = n0 + f;
+    float z[8] = {};
+    if (row < rows) {
+#pragma unroll
+        for (int w = 0; w < ST_WARPS; w++) {
+            const float4 *v = reinterpret_cast<const float4 *>(ring + w * ST_SLOTS * PK_BYTES) +
+                              (row * 128 + f) / 4;
+            const float4 a = v[0], b = v[1];
+            z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
+            z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
+        }
+    }
+    const auto finish = [&](uint32_t r) {
+        if (n >= p.N) return;
+        Operands o;
+        const uint32_t m = m0 + r;
+        float bias[8];
+        load_bias8<BF>(p, e, n, bias);
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] += bias[j];
+        if (p.odt == HCT_B200_F32) {
+            load_operands<HCT_B200_F32>(p, m, n, o);
+            finish8<BF, HCT_B200_F32>(p, z, o, m, n);
+        } else {
+            load_operands<HCT_B200_F16>(p, m, n, o);
+            finish8_any<BF, false>(p, z, o, m, n);
+        }
+    };
+    if (q.split == 1) {
+        if (row < rows) finish(row);
+        return;
+    }
+    // row r is finished by CTA r % split, which receives its parts at
+    // [r / split][source rank]
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (row < rows) {
+        const uint32_t at = smem_u32(recv + ((row / q.split) * q.split + rank) * 128 + f);
+        const uint32_t to = map_to(at, row % q.split);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(z[0]),
+                     "f"(z[1]), "f"(z[2]), "f"(z[3])
+                     : "memory");
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + 16), "f"(z[4]),
+                     "f"(z[5]), "f"(z[6]), "f"(z[7])
+                     : "memory");
+    }
+    cluster_barrier();
+    const uint32_t mine = row * q.split + rank;  // this thread's row, of those that I finish
+    if (mine < rows) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] = 0.0f;
+        for (uint32_t r = 0; r < q.split; r++) {
+            const float4 *v = reinterpret_cast<const float4 *>(recv + (row * q.split + r) * 128 + f);
+            const float4 a = v[0], b = v[1];
+            z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
+            z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
+        }
+        finish(mine);
+    }
+}
+
 // ---- host side --------------------------------------------------------------------
 
 int code_of(cudaError_t e) {
@@ -1315,20 +1583,25 @@ bool tma_rows(const void *base, uint64_t rows, uint64_t ld, uint64_t K) {
 
 inline uint32_t round_to(uint32_t v, uint32_t m) { return (v + m - 1) / m * m; }
 
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &set) {
+    // once per device (64 of them remembered); twice by two threads does no harm
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (set.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+}
+
 template <bool INT4, bool BF, bool PRECISE, bool PAIR>
 cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const UmmaParams &u,
                         uint32_t grid, uint32_t smem, cudaStream_t s) {
     const auto kernel = linear_umma_kernel<INT4, BF, PRECISE, PAIR>;
-    // once per device (64 of them remembered); twice by two threads does no harm
     static std::atomic<uint64_t> set{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    cudaError_t e = allow_smem(kernel, SMEM_LIMIT, set);
     if (e != cudaSuccess) return e;
-    if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT);
-        if (e != cudaSuccess) return e;
-        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(grid);
     c.blockDim = dim3(umma_threads(INT4));
@@ -1428,6 +1701,48 @@ cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaS
     return bf ? launch(no, yes) : launch(no, no);
 }
 
+template <bool BF, int NT>
+cudaError_t launch_stream(const StreamParams &q, uint32_t grid, cudaStream_t s) {
+    static std::atomic<uint64_t> set{0};
+    const auto kernel = linear_int4_stream_kernel<BF, NT>;
+    const uint32_t fixed = ST_WARPS * ST_SLOTS * (PK_BYTES + 8) + 8 * NT * 128 * 4 + 16;
+    cudaError_t e = allow_smem(kernel, fixed + (MAX_EXPERTS + 1) * 8, set);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(ST_THREADS);
+    c.dynamicSmemBytes = fixed + (q.p.E + 1) * 8;
+    c.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = q.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    c.attrs = attr;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, q);
+}
+
+constexpr uint32_t STREAM_ROWS = 16;  // rows (per expert with rows) up to which the stream kernel is taken
+
+cudaError_t run_stream(const LinParams &p, bool bf, cudaStream_t s) {
+    const uint32_t sms = (uint32_t)sm_count(), kbs = (uint32_t)pk_kblocks(p.K);
+    const uint32_t active = std::min(p.E, p.M);
+    const bool two = p.M / active > 8 || (p.E == 1 && p.M > 8);
+    StreamParams q{};
+    q.p = p;
+    q.vec_x = (uintptr_t)p.x % 16 == 0 && (p.M == 1 || p.ldx % 8 == 0);
+    const uint64_t row_tiles = p.E == 1 ? (p.M + (two ? 15 : 7)) / (two ? 16 : 8)
+                                        : p.M / (two ? 16 : 8) + active;
+    const uint64_t tiles = row_tiles * ((p.N + 127) / 128);
+    if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
+    // two CTAs fit an SM; a part keeps at least a block for each warp
+    q.split = 1;
+    while (q.split < 8 && tiles * q.split * 2 <= 2 * sms && kbs >= q.split * 2 * ST_WARPS) q.split *= 2;
+    const uint32_t grid = (uint32_t)tiles * q.split;
+    if (bf) return two ? launch_stream<true, 2>(q, grid, s) : launch_stream<true, 1>(q, grid, s);
+    return two ? launch_stream<false, 2>(q, grid, s) : launch_stream<false, 1>(q, grid, s);
+}
+
 int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     bool nothing = false;
     const int rc = check(a, grouped, &nothing);
@@ -1462,6 +1777,7 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     p.vec_res = rows16(p.res, p.ldres, osz);
     p.vec_out = rows16(p.out, p.ldo, osz);
     const bool bf = a->x_dtype == HCT_B200_BF16, int4 = a->weight_form == HCT_B200_WEIGHT_INT4;
+    if (int4 && p.M <= STREAM_ROWS * std::min(p.E, p.M)) return code_of(run_stream(p, bf, s));
     // the tensor cores take rows that TMA can fetch (and strides that its maps can hold)
     const bool w_ok = int4 || (tma_rows(p.w, p.N, p.ldw, p.K) &&
                                (p.E == 1 || (p.w_stride % 8 == 0 && p.w_stride && p.w_stride < 1ull << 38)));

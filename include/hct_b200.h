@@ -257,8 +257,8 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * do not show; F32 outputs are therefore summed in sections of 256 that are
  * added with rounding.  INT4 weights are (nibble - 8) * scale: rounded to
  * x's type as hct_b200_dequantize_int4 rounds them for 16-bit outputs, and
- * held exactly (as the sum of two values of x's type) for F32 outputs; in F16
- * a weight beyond 65504 is infinite.
+ * held exactly for F32 outputs (and for a few rows of x); beyond 65504 they may
+ * be infinite where x is F16.
  *
  * Strides are in elements.  Rows of x and w that start on 16-byte boundaries
  * take the tensor-core path; others are handled by a slower kernel.  out may
