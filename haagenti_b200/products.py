@@ -11,6 +11,9 @@ its decoded tensors to an external runtime.
 """
 from __future__ import annotations
 
+import struct
+import threading
+
 from . import (F16, BF16, F32, Unsupported, _as_host_u8, _check, _torch)
 from . import _lib as L
 from ._lib import ACT_NONE
@@ -22,9 +25,24 @@ _TYPE: dict = {}  # and back
 _raw_stream = None  # device index -> its current stream's cudaStream_t
 
 
+class _Args(threading.local):
+    """A thread's hct_b200_linear_args, filled by one pack (half the time of
+    setting the fields)."""
+
+    layout = struct.Struct("=15QQIiiiiiii")  # the fields in the header's order
+
+    def __init__(self):
+        self.buffer = bytearray(self.layout.size)
+        self.args = L.LinearArgs.from_buffer(self.buffer)
+
+
+_ARGS = _Args()
+
+
 def _first_call():
     global _raw_stream
     torch = _torch()
+    L.load()
     # the handle alone: torch.cuda.current_stream builds a Stream object, 3 us of a call's 10
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                           lambda i: torch.cuda.current_stream(i).cuda_stream)
@@ -108,9 +126,9 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
     torch = _torch()
     if not _TAG:
         _first_call()
-    if x.dim() != 2 or not x.is_cuda:
-        raise ValueError("x must be a 2-D CUDA tensor (rows, in_features)")
     dev = x.get_device()
+    if dev < 0 or x.dim() != 2:
+        raise ValueError("x must be a 2-D CUDA tensor (rows, in_features)")
     m, k = x.shape
     xt = x.dtype
     x_tag = _TAG.get(xt)
@@ -144,7 +162,7 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
         raise ValueError(f"x has {k} features, the weight {wk}")
     if wt.get_device() != dev:
         raise ValueError(f"the weight is on {wt.device}, x on {x.device}")
-    bits, off_ptr = 32, None
+    bits, off_ptr = 32, 0
     if offsets is None:
         if experts is not None:
             raise ValueError("a weight with experts needs grouped_linear")
@@ -168,7 +186,7 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
             raise ValueError(f"out_dtype must be F32, F16 or BF16, got {out_dtype}")
     ot = _TYPE[tag]
     shape = (m, n)
-    bias_tag, bias_ptr, gate_ptr, res_ptr, ldg, ldr = x_tag, None, None, None, 0, 0
+    bias_tag, bias_ptr, gate_ptr, res_ptr, ldg, ldr = x_tag, 0, 0, 0, 0, 0
     grads = x.requires_grad or wt.requires_grad
     if bias is not None:
         want = (n,) if offsets is None else (experts, n)
@@ -192,25 +210,29 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
     if grads and torch.is_grad_enabled():
         raise Unsupported(L.UNSUPPORTED, "the products have no backward pass: detach the tensors "
                                          "or call under torch.no_grad()")
-    lib = L.load()
+    lib = L._lib
     fn = lib.hct_b200_linear if offsets is None else lib.hct_b200_grouped_linear
-
-    def call(raw):
-        o = out if out is not None else torch.empty(shape, dtype=ot, device=x.device)
-        _check(fn(L.LinearArgs(m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride, bias_ptr,
-                               gate_ptr, ldg, res_ptr, ldr, o.data_ptr(), o.stride(0), off_ptr,
-                               experts, bits, x_tag, form, bias_tag, tag, activation, 0), raw))
-        return o
-
-    if stream is None and torch.cuda.current_device() == dev:
-        return call(_raw_stream(dev))
+    here = torch.cuda.current_device() == dev
+    if here and stream is None:
+        if out is None:
+            out = x.new_empty(shape) if ot is xt else x.new_empty(shape, dtype=ot)
+        a = _ARGS
+        a.layout.pack_into(a.buffer, 0, m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride,
+                           bias_ptr, gate_ptr, ldg, res_ptr, ldr, out.data_ptr(), out.stride(0),
+                           off_ptr, experts, bits, x_tag, form, bias_tag, tag, activation, 0)
+        rc = fn(a.args, _raw_stream(dev))
+        if rc:
+            _check(rc)
+        return out
     with torch.cuda.device(dev):
-        if stream is None or stream == torch.cuda.current_stream():
-            return call(_raw_stream(dev))
+        current = torch.cuda.current_stream()
+        if stream is None or stream == current:
+            return _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, out,
+                            None)
         if stream.device.index != dev:
             raise ValueError(f"the stream belongs to {stream.device}, x to {x.device}")
         with torch.cuda.stream(stream):
-            o = call(stream.cuda_stream)
+            o = _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, out, None)
         # the caller's tensors are read on a stream that their allocator does not know of
         for t in (x, wt, offsets, bias, gate, residual, out):
             if t is not None:
