@@ -80,6 +80,18 @@ __global__ void int4_weight_pack_kernel(const uint8_t *__restrict__ data, uint64
     }
 }
 
+// Division by a number known on the host, of values below 2^31: a product and a
+// shift in place of the 35 dependent instructions of a division.
+struct Divisor {
+    uint32_t d, mul, shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t n) : d(n), shift(0) {
+        while (shift < 31 && (1ull << shift) < n) shift++;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - n)) / n + 1);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t v) const { return (__umulhi(v, mul) + v) >> shift; }
+};
+
 // ---- what every kernel is given -------------------------------------------------
 
 struct LinParams {
@@ -92,13 +104,19 @@ struct LinParams {
     int vec_gate, vec_res, vec_out;  // rows start on 16-byte boundaries
 };
 
-// The groups: off[e] .. off[e + 1] are the rows of expert e, first[e] is the
-// number of `tile`-row tiles of the experts before it and first[E] their total.
-// Offsets are clamped to [0, M] and to the largest before them, so that groups
-// never overlap; without offsets the one expert owns every row.  Called by one
-// whole warp; both arrays are shared memory, of E + 1 entries.
-__device__ __forceinline__ void scan_groups(const LinParams &p, uint32_t tile, uint32_t *first,
-                                            uint32_t *off) {
+// The groups, in shared memory: off[e] .. off[e + 1] are the rows of expert e,
+// first[e] is the number of row tiles of the experts before it (first[E] their
+// total) and per[e] the rows of each of its tiles: dealt out evenly, in whole
+// multiples of 16 up to `tile.d`.  Offsets are clamped to [0, M] and to the
+// largest before them, so that groups never overlap; without offsets the one
+// expert owns every row.  Called by one whole warp.
+struct Groups {
+    uint32_t *first, *off, *per;
+    __device__ __forceinline__ Groups(uint32_t *at, uint32_t E) : first(at), off(at + E + 1), per(off + E + 1) {}
+};
+constexpr uint32_t groups_bytes(uint32_t E) { return (3 * E + 2) * 4; }
+
+__device__ __forceinline__ void scan_groups(const LinParams &p, const Divisor &tile, const Groups &g) {
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t most = 0;  // largest offset so far
     for (uint32_t i0 = 0; i0 <= p.E; i0 += 32) {
@@ -116,24 +134,28 @@ __device__ __forceinline__ void scan_groups(const LinParams &p, uint32_t tile, u
             const uint32_t w = __shfl_up_sync(0xffffffffu, o, d);
             if (lane >= (uint32_t)d) o = max(o, w);
         }
-        if (i <= p.E) off[i] = o;
+        if (i <= p.E) g.off[i] = o;
         most = __shfl_sync(0xffffffffu, o, 31);
     }
     __syncwarp();
     uint32_t base = 0;
     for (uint32_t e0 = 0; e0 < p.E; e0 += 32) {
         const uint32_t e = e0 + lane;
-        const uint32_t c = e < p.E ? (off[e + 1] - off[e] + tile - 1) / tile : 0;
+        const uint32_t m = e < p.E ? g.off[e + 1] - g.off[e] : 0;
+        const uint32_t c = tile.of(m + tile.d - 1);
         uint32_t sum = c;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t w = __shfl_up_sync(0xffffffffu, sum, d);
             if (lane >= (uint32_t)d) sum += w;
         }
-        if (e < p.E) first[e] = base + sum - c;
+        if (e < p.E) {
+            g.first[e] = base + sum - c;
+            g.per[e] = c > 1 ? ((m + c - 1) / c + 15) / 16 * 16 : m;
+        }
         base += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) first[p.E] = base;
+    if (lane == 0) g.first[p.E] = base;
     __syncwarp();
 }
 
@@ -180,17 +202,6 @@ __device__ __forceinline__ float activate(float z, int act) {
     }
 }
 
-__device__ __forceinline__ float load_out_type(const void *p, uint64_t i, int dt) {
-    if (dt == HCT_B200_F32) return reinterpret_cast<const float *>(p)[i];
-    const uint16_t v = reinterpret_cast<const uint16_t *>(p)[i];
-    return dt == HCT_B200_F16 ? h2f(v) : bf2f(v);
-}
-__device__ __forceinline__ void store_out(void *p, uint64_t i, int dt, float v) {
-    if (dt == HCT_B200_F32) reinterpret_cast<float *>(p)[i] = v;
-    else if (dt == HCT_B200_F16) reinterpret_cast<__half *>(p)[i] = __float2half_rn(v);
-    else reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
-
 template <bool BF>
 __device__ __forceinline__ float bias_of(const LinParams &p, uint32_t e, uint32_t n) {
     if (!p.bias) return 0.0f;
@@ -199,94 +210,7 @@ __device__ __forceinline__ float bias_of(const LinParams &p, uint32_t e, uint32_
                       : from16<BF>(reinterpret_cast<const uint16_t *>(p.bias)[i]);
 }
 
-// The epilogue of one output: z is the sum plus bias.
-template <bool BF>
-__device__ __forceinline__ void finish(const LinParams &p, uint32_t m, uint32_t n, float z) {
-    float y = activate(z, p.act);
-    if (p.gate)
-        y *= from16<BF>(reinterpret_cast<const uint16_t *>(p.gate)[(uint64_t)m * p.ldgate + n]);
-    if (p.res) y += load_out_type(p.res, (uint64_t)m * p.ldres + n, p.odt);
-    store_out(p.out, (uint64_t)m * p.ldo + n, p.odt, y);
-}
-
 __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has expired
-
-// ---- plain kernel: any alignment, any stride ------------------------------------
-//
-// 32 rows x 64 features per CTA, 32-wide K steps through shared memory, f32
-// multiply-adds (2 x 4 outputs per thread).  Every element is loaded by itself
-// and checked against its bounds.
-constexpr int SM_M = 32, SM_N = 64, SM_K = 32, SM_THREADS = 256;
-
-template <bool BF, bool INT4>
-__global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParams p) {
-    __shared__ uint32_t first[MAX_EXPERTS + 1], off[MAX_EXPERTS + 1];
-    __shared__ float xs[SM_K][SM_M + 1], ws[SM_K][SM_N + 1];
-    const uint32_t tid = threadIdx.x;
-    if (tid < 32) scan_groups(p, SM_M, first, off);
-    __syncthreads();
-    const uint32_t n_tiles = (p.N + SM_N - 1) / SM_N;
-    const uint64_t tiles = (uint64_t)first[p.E] * n_tiles;
-    const uint32_t tn = tid % 16, tm = tid / 16;
-    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const uint32_t mt = (uint32_t)(t / n_tiles), n0 = (uint32_t)(t % n_tiles) * SM_N;
-        const uint32_t e = expert_of(first, p.E, mt);
-        const uint32_t hi = off[e + 1], m0 = off[e] + (mt - first[e]) * SM_M;
-        float acc[2][4] = {};
-        for (uint32_t k0 = 0; k0 < p.K; k0 += SM_K) {
-            for (uint32_t i = tid; i < SM_M * SM_K; i += SM_THREADS) {
-                const uint32_t k = k0 + i % SM_K, m = m0 + i / SM_K;
-                xs[i % SM_K][i / SM_K] =
-                    k < p.K && m < hi
-                        ? from16<BF>(reinterpret_cast<const uint16_t *>(p.x)[(uint64_t)m * p.ldx + k])
-                        : 0.0f;
-            }
-            for (uint32_t i = tid; i < SM_N * SM_K; i += SM_THREADS) {
-                const uint32_t k = k0 + i % SM_K, n = n0 + i / SM_K;
-                float v = 0.0f;
-                if (k < p.K && n < p.N) {
-                    if (INT4) {
-                        const uint64_t kb = pk_kblocks(p.K);
-                        const uint64_t per = (uint64_t)((p.N + PK_ROWS - 1) / PK_ROWS) * kb;
-                        const uint8_t *b = reinterpret_cast<const uint8_t *>(p.w) +
-                                           (e * per + n / PK_ROWS * kb + k / PK_COLS) * PK_BYTES;
-                        const uint32_t in = (k / 32 % 2) * PK_ROWS + n % PK_ROWS, c = k / 8 % 4;
-                        const uint32_t word = *reinterpret_cast<const uint32_t *>(b + in * 16 + c * 4);
-                        const uint32_t q = word >> (4 * (k % 8 / 2) + 16 * (k % 2)) & 15u;
-                        v = (float)((int)q - 8) *
-                            h2f(*reinterpret_cast<const uint16_t *>(
-                                b + PK_NIB + (k / 32 % 2 * PK_ROWS + pk_scale_at(n % PK_ROWS)) * 2));
-                    } else {
-                        v = from16<BF>(reinterpret_cast<const uint16_t *>(
-                            p.w)[(uint64_t)e * p.w_stride + (uint64_t)n * p.ldw + k]);
-                    }
-                }
-                ws[i % SM_K][i / SM_K] = v;
-            }
-            __syncthreads();
-#pragma unroll 8
-            for (int k = 0; k < SM_K; k++) {
-                float a[2], b[4];
-#pragma unroll
-                for (int i = 0; i < 2; i++) a[i] = xs[k][tm + 16 * i];
-#pragma unroll
-                for (int j = 0; j < 4; j++) b[j] = ws[k][tn + 16 * j];
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t m = m0 + tm + 16 * i, n = n0 + tn + 16 * j;
-                if (m < hi && n < p.N) finish<BF>(p, m, n, acc[i][j] + bias_of<BF>(p, e, n));
-            }
-    }
-}
 
 // ---- tensor-core kernel ---------------------------------------------------------
 //
@@ -304,8 +228,10 @@ __global__ void __launch_bounds__(SM_THREADS) linear_plain_kernel(const LinParam
 //               accumulators (TMEM lanes = features) through shared memory into
 //               runs of 8 features, so that outputs, gate and residual move in
 //               16-byte pieces of a row
-//   warps 12-23 INT4 only: three groups of 128 threads dequantise every third
-//               K step, a thread per weight row, into the 128B-swizzled A tile
+//   warps 12-23 INT4: three groups of 128 threads dequantise every third K step,
+//               a thread per weight row, into the 128B-swizzled A tile.  Dense
+//               rows that TMA cannot fetch (unaligned starts, odd strides): they
+//               copy both operands by plain loads
 //
 // PAIR: where whole tiles of rows keep every SM busy, two CTAs share one tile of
 // 256 features (cta_group::2): each holds the weights of its 128 features and
@@ -341,6 +267,7 @@ struct UmmaParams {
     uint32_t stages, raw_stages;
     uint32_t tmem_cols, tmem_stride;
     uint32_t split;   // CTAs per cluster, each a part of K
+    Divisor tile, nt, band;  // by bn, by feature tiles, by RASTER x feature tiles
 };
 
 struct Ctl {
@@ -589,23 +516,17 @@ struct Tile {
     uint32_t e, m0, rows, n0;
 };
 template <uint32_t FEATURES>
-__device__ __forceinline__ Tile tile_at(const UmmaParams &u, const uint32_t *first,
-                                        const uint32_t *off, uint32_t t) {
-    const LinParams &p = u.p;
-    const uint32_t nt = (p.N + FEATURES - 1) / FEATURES;
+__device__ __forceinline__ Tile tile_at(const UmmaParams &u, const Groups &g, uint32_t t) {
     Tile r;
-    r.e = expert_of(first, p.E, t / nt);
-    const uint32_t lo = off[r.e], hi = off[r.e + 1], m = hi - lo, mts = (m + u.bn - 1) / u.bn;
-    // rows dealt out evenly, in whole instruction widths
-    const uint32_t per = ((m + mts - 1) / mts + 15) / 16 * 16;
-    // groups of RASTER row tiles; within one, the row tiles of a feature tile
-    // run next to each other, so that the tiles in flight share x and w in L2
-    const uint32_t q = t - first[r.e] * nt;
-    const uint32_t grp = q / (RASTER * nt), in = q - grp * RASTER * nt;
-    const uint32_t width = min(RASTER, mts - grp * RASTER);
-    const uint32_t mt = grp * RASTER + in % width;
-    r.n0 = in / width * FEATURES;
-    r.m0 = lo + mt * per;
+    r.e = u.p.E > 1 ? expert_of(g.first, u.p.E, u.nt.of(t)) : 0;
+    const uint32_t lo = g.off[r.e], hi = g.off[r.e + 1], per = g.per[r.e], first = g.first[r.e];
+    // bands of RASTER row tiles; within one, the row tiles of a feature tile run
+    // next to each other, so that the tiles in flight share x and w in L2
+    const uint32_t q = t - first * u.nt.d, band = u.band.of(q), in = q - band * u.band.d;
+    const uint32_t width = min(RASTER, g.first[r.e + 1] - first - band * RASTER);
+    const uint32_t ft = width == RASTER ? in / RASTER : width == 1 ? in : in / width;
+    r.n0 = ft * FEATURES;
+    r.m0 = lo + (band * RASTER + in - ft * width) * per;
     r.rows = min(per, hi - r.m0);
     return r;
 }
@@ -832,16 +753,22 @@ __device__ __forceinline__ void load_bias8(const LinParams &p, uint32_t e, uint3
     for (int j = 0; j < 8; j++) bias[j] = n + j < p.N ? bias_of<BF>(p, e, n + j) : 0.0f;
 }
 
-constexpr int umma_threads(bool int4) { return int4 ? 768 : 384; }
+// Where the operands come from: dense matrices by TMA, packed INT4 weights (x by
+// TMA), or dense matrices of any stride and alignment, copied by warps.
+enum { FORM_DENSE = 0, FORM_INT4 = 1, FORM_ANY = 2 };
+constexpr int umma_threads(int form) { return form == FORM_DENSE ? 384 : 768; }
 // rows per tile at most: a thread of the epilogue keeps half of them as f32 sums where PRECISE
-__host__ __device__ constexpr uint32_t max_rows(bool int4, bool precise) { return precise ? (int4 ? 64 : 128) : 256; }
+__host__ __device__ constexpr uint32_t max_rows(int form, bool precise) {
+    return precise ? (form == FORM_DENSE ? 128 : 64) : 256;
+}
 
-template <bool INT4, bool BF, bool PRECISE, bool PAIR>
-__global__ void __launch_bounds__(umma_threads(INT4), 1)
+template <int FORM, bool BF, bool PRECISE, bool PAIR>
+__global__ void __launch_bounds__(umma_threads(FORM), 1)
     linear_umma_kernel(const __grid_constant__ CUtensorMap tmX,
                        const __grid_constant__ CUtensorMap tmW, const __grid_constant__ UmmaParams u) {
+    constexpr bool INT4 = FORM == FORM_INT4, ANY = FORM == FORM_ANY, TMA_W = FORM == FORM_DENSE;
     constexpr uint32_t A_PARTS = INT4 && PRECISE ? 2 : 1;
-    constexpr uint32_t GROUPS = 3;  // of dequantising warps
+    constexpr uint32_t GROUPS = 3;  // of dequantising or loading warps
     constexpr uint32_t FEATURES = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -850,7 +777,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     uint8_t *raw = smem + (size_t)stages * stage_bytes;
     uint8_t *epi = raw + (size_t)u.raw_stages * PK_BYTES;
     Ctl *ctl = reinterpret_cast<Ctl *>(epi + EPI_BYTES);
-    uint32_t *first = reinterpret_cast<uint32_t *>(ctl + 1), *off = first + p.E + 1;
+    const Groups groups(reinterpret_cast<uint32_t *>(ctl + 1), p.E);
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0) {
@@ -880,7 +807,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
     }
     let_next_kernel_start();
     after_previous_kernel();
-    if (warp == 2) scan_groups(p, u.bn, first, off);
+    if (warp == 2) scan_groups(p, u.tile, groups);
     __syncthreads();
     if (PAIR) cluster_barrier();  // the other CTA's barriers are set up too
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -891,28 +818,32 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         atomicExch(&ctl->abort, 1);
     };
 
-    const uint32_t tiles = uniform(first[p.E]) * ((p.N + FEATURES - 1) / FEATURES);
+    const uint32_t tiles = uniform(groups.first[p.E]) * u.nt.d;
     // clusters are consecutive CTAs: the parts of a K range, or a pair
-    const uint32_t rank = blockIdx.x % u.split, side = PAIR ? blockIdx.x & 1u : 0u;
-    const uint32_t t0 = blockIdx.x / (PAIR ? 2 : u.split), step = gridDim.x / (PAIR ? 2 : u.split);
-    const uint32_t kbs = (p.K + BK - 1) / BK;
-    const uint32_t kb0 = (uint32_t)((uint64_t)kbs * rank / u.split);
-    const uint32_t kb1 = (uint32_t)((uint64_t)kbs * (rank + 1) / u.split);
+    const uint32_t rank = u.split > 1 ? blockIdx.x % u.split : 0, side = PAIR ? blockIdx.x & 1u : 0u;
+    const uint32_t t0 = PAIR ? blockIdx.x / 2 : u.split > 1 ? blockIdx.x / u.split : blockIdx.x;
+    const uint32_t step = PAIR ? gridDim.x / 2 : gridDim.x;  // a split has one tile per cluster
+    const uint32_t kbs = max((p.K + BK - 1) / BK, 1u);
+    uint32_t kb0 = 0, kb1 = kbs;
+    if (u.split > 1) {  // below 2^25 x 8
+        kb0 = kbs * rank / u.split;
+        kb1 = kbs * (rank + 1) / u.split;
+    }
     const uint32_t sect = PRECISE ? SECTION : kb1 - kb0;  // K steps per accumulation
 
     // The producers and the MMA warp run whole (their addresses and descriptors
     // are warp-uniform); one elected lane issues.
-    if (warp == 0) {
+    if (!ANY && warp == 0) {
         Ring at(stages);
         uint32_t issued = 0;
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            const Tile c = tile_at<FEATURES>(u, groups, t);
             // each CTA of a pair holds its 128 features and half of the tile's rows,
             // and both copies complete on the leader's barrier
             const uint32_t held = (c.rows + 15) / 16 * 16 / CTAS;
             const uint32_t boxes = (held + u.xbox - 1) / u.xbox;
-            const uint32_t bytes = (boxes * u.xbox * 128 + (INT4 ? 0 : A_BYTES)) * CTAS;
+            const uint32_t bytes = (boxes * u.xbox * 128 + (TMA_W ? A_BYTES : 0)) * CTAS;
             const int m0 = (int)(c.m0 + side * held), n0 = (int)(c.n0 + side * 128);
             for (uint32_t kb = kb0; kb < kb1; kb++, at.step()) {
                 ok = mbar_wait_warp(smem_u32(&ctl->empty[at.slot]), at.pass ^ 1u, &ctl->abort);
@@ -923,7 +854,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                     uint32_t fb = smem_u32(&ctl->xfull[at.slot]);
                     if (side == 0) mbar_expect_tx(fb, bytes);
                     if (PAIR) fb = map_to(fb, 0);
-                    if (!INT4) tma_3d<PAIR>(sa, &tmW, fb, (int)(kb * BK), n0, (int)c.e);
+                    if (TMA_W) tma_3d<PAIR>(sa, &tmW, fb, (int)(kb * BK), n0, (int)c.e);
                     for (uint32_t b = 0; b < boxes; b++)
                         tma_2d<PAIR>(sb + b * u.xbox * 128, &tmX, fb, (int)(kb * BK),
                                      m0 + (int)(b * u.xbox));
@@ -939,11 +870,11 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         const uint32_t idesc0 =
             (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((FEATURES / 16) << 24);
         // INT4: half of the lanes wait for the x tile, half for the weights
-        const uint32_t full = smem_u32(INT4 && lane >= 16 ? ctl->afull : ctl->xfull);
+        const uint32_t full = smem_u32(ANY || (INT4 && lane >= 16) ? ctl->afull : ctl->xfull);
         Ring at(stages), acc(2);
         bool ok = true;
         for (uint32_t t = t0; side == 0 && ok && t < tiles; t += step) {
-            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            const Tile c = tile_at<FEATURES>(u, groups, t);
             const uint32_t idesc = uniform(idesc0 | ((c.rows + 15) / 16 * 2) << 17);
             for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
                 const uint32_t end = min(kb + sect, kb1), from = kb;
@@ -982,7 +913,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         uint32_t issued = 0;
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            const Tile c = tile_at<FEATURES>(u, groups, t);
             // a pair's second half may lie past the last features: any block will do there
             const uint64_t block = (uint64_t)c.e * nt + min(c.n0 / 128 + side, nt - 1);
             const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) + (block * kbs + kb0) * PK_BYTES;
@@ -1046,15 +977,65 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
                 mbar_arrive(smem_u32(&ctl->rempty[in.slot]));
             }
         }
+    } else if (ANY && warp >= 12) {
+        // this group's K steps: a warp copies 32 rows of w and a quarter of the rows of
+        // x, a row at a time, two values per lane
+        const uint32_t group = (warp - 12) >> 2, part = (warp - 12) & 3u, col = lane * 2;
+        Ring to(stages, group);
+        uint32_t turn = group;  // K steps until the group's next
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += step) {
+            const Tile c = tile_at<FEATURES>(u, groups, t);
+            const uint16_t *w = reinterpret_cast<const uint16_t *>(p.w) + c.e * p.w_stride;
+            const uint16_t *x = reinterpret_cast<const uint16_t *>(p.x);
+            const uint32_t xrows = (c.rows + 15) / 16 * 16, quarter = xrows / 4;
+            for (uint32_t kb = kb0; kb < kb1; kb++) {
+                if (turn) {
+                    turn--;
+                    continue;
+                }
+                turn = GROUPS - 1;
+                ok = mbar_wait_warp(smem_u32(&ctl->empty[to.slot]), to.pass ^ 1u, &ctl->abort);
+                if (!ok) break;
+                uint8_t *a = smem + (size_t)to.slot * stage_bytes;
+                const uint32_t k = kb * BK + col;
+                const auto copy = [&](const uint16_t *src, uint64_t ld, uint32_t row0, uint32_t live,
+                                      uint32_t r0, uint32_t count, uint8_t *dst) {
+                    for (uint32_t i = 0; i < count; i += 4) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) {
+                            const uint32_t r = r0 + i + j;
+                            const uint16_t *q = src + (uint64_t)(row0 + r) * ld + k;
+                            v[j] = r < live && k < p.K ? q[0] : 0u;
+                            if (r < live && k + 1 < p.K) v[j] |= (uint32_t)q[1] << 16;
+                        }
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) {
+                            const uint32_t r = r0 + i + j;
+                            *reinterpret_cast<uint32_t *>(
+                                dst + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4) = v[j];
+                        }
+                    }
+                };
+                copy(w, p.ldw, c.n0, p.N - c.n0, part * 32, 32, a);
+                copy(x, p.ldx, c.m0, c.rows, part * quarter, quarter, a + A_BYTES);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->afull[to.slot]));
+                to.step(GROUPS);
+            }
+        }
+        if (!ok) give_up();
     } else if (warp >= 4 && warp < 12) {
-        constexpr int CHUNKS = max_rows(INT4, PRECISE) / 32;  // of 16 rows, per set
+        constexpr int CHUNKS = max_rows(FORM, PRECISE) / 32;  // of 16 rows, per set
         const uint32_t set = (warp - 4) >> 2, q = warp & 3u, id = q * 32 + lane;
         float *part = reinterpret_cast<float *>(smem);  // split: [rows of x][128 features]
         float *stage = reinterpret_cast<float *>(epi + set * (EPI_BYTES / 2));
         Ring acc(2);
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
-            const Tile c = tile_at<FEATURES>(u, first, off, t);
+            const Tile c = tile_at<FEATURES>(u, groups, t);
             const uint32_t n = c.n0 + side * 128 + id % 16 * 8;
             float bias[8];
             if (u.split == 1) load_bias8<BF>(p, c.e, n, bias);
@@ -1131,7 +1112,7 @@ __global__ void __launch_bounds__(umma_threads(INT4), 1)
         __syncwarp();
         cluster_barrier();
         if (t0 < tiles && !aborted()) {
-            const Tile c = tile_at<FEATURES>(u, first, off, t0);
+            const Tile c = tile_at<FEATURES>(u, groups, t0);
             const uint32_t j0 = c.rows * rank / u.split, j1 = c.rows * (rank + 1) / u.split;
             const uint32_t f = threadIdx.x % 16 * 8, n = c.n0 + f, base = smem_u32(smem);
             if (n < p.N) {
@@ -1210,8 +1191,9 @@ constexpr int ST_WARPS = 8, ST_THREADS = ST_WARPS * 32, ST_SLOTS = 2;
 
 struct StreamParams {
     LinParams p;
-    uint32_t split;
-    int vec_x;  // rows of x start on 16-byte boundaries
+    uint32_t split, shift;  // CTAs per cluster: 1 << shift
+    int vec_x;              // rows of x start on 16-byte boundaries
+    Divisor tile, nt;       // by 8 NT rows, by feature tiles
 };
 
 // d = a b of m16n8k16, and d += a b.
@@ -1290,8 +1272,8 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
     uint8_t *ring = st_smem;                                                   // [warp][slot]
     float *recv = reinterpret_cast<float *>(ring + ST_WARPS * ST_SLOTS * PK_BYTES);  // [ROWS][128]
     uint64_t *full = reinterpret_cast<uint64_t *>(recv + ROWS * 128);           // [warp][slot]
-    uint32_t *first = reinterpret_cast<uint32_t *>(full + ST_WARPS * ST_SLOTS), *off = first + p.E + 1;
-    int *abort = reinterpret_cast<int *>(off + p.E + 1);
+    int *abort = reinterpret_cast<int *>(full + ST_WARPS * ST_SLOTS);
+    const Groups groups(reinterpret_cast<uint32_t *>(abort + 2), p.E);
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST_WARPS * ST_SLOTS; i++) mbar_init(smem_u32(&full[i]), 1);
@@ -1300,14 +1282,14 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     after_previous_kernel();
-    if (warp == 1) scan_groups(p, ROWS, first, off);
+    if (warp == 1) scan_groups(p, q.tile, groups);
     __syncthreads();
     // the cluster's CTAs are all running before any of them writes to another
     if (q.split > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
-    const uint32_t nt = (p.N + 127) / 128, kbs = (uint32_t)pk_kblocks(p.K);
-    const uint32_t rank = blockIdx.x % q.split, t = blockIdx.x / q.split;
-    const bool work = t < first[p.E] * nt;  // of the whole cluster alike
+    const uint32_t nt = q.nt.d, kbs = (uint32_t)pk_kblocks(p.K);
+    const uint32_t rank = blockIdx.x & (q.split - 1), t = blockIdx.x >> q.shift;
+    const bool work = t < groups.first[p.E] * nt;  // of the whole cluster alike
     uint32_t e = 0, m0 = 0, hi = 0, n0 = 0;
     float acc[8][NT][4];
 #pragma unroll
@@ -1318,12 +1300,12 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
             for (int j = 0; j < 4; j++) acc[i][c][j] = 0.0f;
     bool ok = true;
     if (work) {
-        e = expert_of(first, p.E, t / nt);
-        hi = off[e + 1];
-        m0 = off[e] + (t / nt - first[e]) * ROWS;
-        n0 = t % nt * 128;
-        const uint32_t kb0 = (uint32_t)((uint64_t)kbs * rank / q.split);
-        const uint32_t kb1 = (uint32_t)((uint64_t)kbs * (rank + 1) / q.split);
+        const uint32_t rt = q.nt.of(t);
+        e = p.E > 1 ? expert_of(groups.first, p.E, rt) : 0;
+        hi = groups.off[e + 1];
+        m0 = groups.off[e] + (rt - groups.first[e]) * ROWS;
+        n0 = (t - rt * nt) * 128;
+        const uint32_t kb0 = kbs * rank >> q.shift, kb1 = kbs * (rank + 1) >> q.shift;
         const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
                              ((uint64_t)e * nt + n0 / 128) * kbs * PK_BYTES;
         uint8_t *mine = ring + warp * ST_SLOTS * PK_BYTES;
@@ -1457,8 +1439,8 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
     // [r / split][source rank]
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (row < rows) {
-        const uint32_t at = smem_u32(recv + ((row / q.split) * q.split + rank) * 128 + f);
-        const uint32_t to = map_to(at, row % q.split);
+        const uint32_t at = smem_u32(recv + ((row >> q.shift << q.shift) + rank) * 128 + f);
+        const uint32_t to = map_to(at, row & (q.split - 1));
         asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(z[0]),
                      "f"(z[1]), "f"(z[2]), "f"(z[3])
                      : "memory");
@@ -1467,12 +1449,14 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
                      : "memory");
     }
     cluster_barrier();
-    const uint32_t mine = row * q.split + rank;  // this thread's row, of those that I finish
+    const uint32_t mine = (row << q.shift) + rank;  // this thread's row, of those that I finish
     if (mine < rows) {
 #pragma unroll
         for (int j = 0; j < 8; j++) z[j] = 0.0f;
-        for (uint32_t r = 0; r < q.split; r++) {
-            const float4 *v = reinterpret_cast<const float4 *>(recv + (row * q.split + r) * 128 + f);
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) {
+            if (r >= q.split) break;
+            const float4 *v = reinterpret_cast<const float4 *>(recv + ((row << q.shift) + r) * 128 + f);
             const float4 a = v[0], b = v[1];
             z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
             z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
@@ -1648,16 +1632,16 @@ cudaError_t allow_smem(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &set
     return e;
 }
 
-template <bool INT4, bool BF, bool PRECISE, bool PAIR>
+template <int FORM, bool BF, bool PRECISE, bool PAIR>
 cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const UmmaParams &u,
                         uint32_t grid, uint32_t smem, cudaStream_t s) {
-    const auto kernel = linear_umma_kernel<INT4, BF, PRECISE, PAIR>;
+    const auto kernel = linear_umma_kernel<FORM, BF, PRECISE, PAIR>;
     static std::atomic<uint64_t> set{0};
     cudaError_t e = allow_smem(kernel, SMEM_LIMIT, set);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(grid);
-    c.blockDim = dim3(umma_threads(INT4));
+    c.blockDim = dim3(umma_threads(FORM));
     c.dynamicSmemBytes = smem;
     c.stream = s;
     cudaLaunchAttribute attr[2];
@@ -1687,16 +1671,17 @@ uint32_t tile_rows(uint32_t M, uint32_t nt, uint32_t units, uint32_t cap) {
 
 // Pair or single, tile height, split and ring depths of a call on the
 // tensor-core kernel.
-cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaStream_t s) {
+cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaStream_t s) {
+    const bool int4 = form == FORM_INT4, any = form == FORM_ANY;
     const bool precise = p.odt == HCT_B200_F32;
-    const uint32_t sms = (uint32_t)sm_count(), cap = max_rows(int4, precise);
-    const uint32_t kbs = (p.K + BK - 1) / BK;
+    const uint32_t sms = (uint32_t)sm_count(), cap = max_rows(form, precise);
+    const uint32_t kbs = std::max((p.K + BK - 1) / BK, 1u);
     const uint32_t active = std::min(p.E, p.M), per_expert = p.M / active;
     UmmaParams u{};
     u.p = p;
     u.split = 1;
     // pairs where tiles of 256 features and full height keep every pair busy
-    const bool pair = !precise && per_expert >= 192 &&
+    const bool pair = !precise && !any && per_expert >= 192 &&
                       (uint64_t)((p.N + 255) / 256) * (p.M / 256) * 2 >= sms;
     const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128, units = pair ? sms / 2 : sms;
     uint64_t row_tiles;  // at most
@@ -1725,43 +1710,48 @@ cudaError_t run_umma(const LinParams &p, bool grouped, bool int4, bool bf, cudaS
     const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn / (pair ? 2 : 1) * 128;
     u.raw_stages = int4 ? 10 : 0;
     const uint32_t fixed =
-        1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) + (p.E + 1) * 8;
+        1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) + groups_bytes(p.E);
+    u.tile = Divisor(u.bn);
+    u.nt = Divisor(nt);
+    u.band = Divisor(nt * RASTER);
     u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
     const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
 
-    alignas(64) CUtensorMap tx, tw;
-    if (!operand_map(&tx, bf, p.x, p.K, p.M, p.M == 1 ? round_to(p.K, 8) : p.ldx, 0, 0, u.xbox))
+    alignas(64) CUtensorMap tx{}, tw{};
+    if (!any && !operand_map(&tx, bf, p.x, p.K, p.M, p.M == 1 ? round_to(p.K, 8) : p.ldx, 0, 0, u.xbox))
         return cudaErrorInvalidValue;
-    if (int4) {
-        tw = tx;
-    } else {
+    if (form == FORM_DENSE) {
         const uint64_t ld = p.N == 1 ? round_to(p.K, 8) : p.ldw;
         if (!operand_map(&tw, bf, p.w, p.K, p.N, ld, p.E, p.E == 1 ? ld * p.N : p.w_stride, 128))
             return cudaErrorInvalidValue;
     }
-    const auto launch = [&](auto is_int4, auto is_bf) {
-        constexpr bool I = decltype(is_int4)::value, B = decltype(is_bf)::value;
-        if (precise) return launch_umma<I, B, true, false>(tx, tw, u, grid, smem, s);
-        if (pair) return launch_umma<I, B, false, true>(tx, tw, u, grid, smem, s);
-        return launch_umma<I, B, false, false>(tx, tw, u, grid, smem, s);
+    const auto launch = [&](auto form_, auto bf_) {
+        constexpr int F = decltype(form_)::value;
+        constexpr bool B = decltype(bf_)::value;
+        if (precise) return launch_umma<F, B, true, false>(tx, tw, u, grid, smem, s);
+        if constexpr (F != FORM_ANY)
+            if (pair) return launch_umma<F, B, false, true>(tx, tw, u, grid, smem, s);
+        return launch_umma<F, B, false, false>(tx, tw, u, grid, smem, s);
     };
-    const std::true_type yes;
-    const std::false_type no;
-    if (int4) return bf ? launch(yes, yes) : launch(yes, no);
-    return bf ? launch(no, yes) : launch(no, no);
+    const auto typed = [&](auto form_) {
+        return bf ? launch(form_, std::true_type()) : launch(form_, std::false_type());
+    };
+    if (int4) return typed(std::integral_constant<int, FORM_INT4>());
+    if (any) return typed(std::integral_constant<int, FORM_ANY>());
+    return typed(std::integral_constant<int, FORM_DENSE>());
 }
 
 template <bool BF, int NT>
 cudaError_t launch_stream(const StreamParams &q, uint32_t grid, cudaStream_t s) {
     static std::atomic<uint64_t> set{0};
     const auto kernel = linear_int4_stream_kernel<BF, NT>;
-    const uint32_t fixed = ST_WARPS * ST_SLOTS * (PK_BYTES + 8) + 8 * NT * 128 * 4 + 16;
-    cudaError_t e = allow_smem(kernel, fixed + (MAX_EXPERTS + 1) * 8, set);
+    const uint32_t fixed = ST_WARPS * ST_SLOTS * (PK_BYTES + 8) + 8 * NT * 128 * 4 + 8;
+    cudaError_t e = allow_smem(kernel, fixed + groups_bytes(MAX_EXPERTS), set);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(grid);
     c.blockDim = dim3(ST_THREADS);
-    c.dynamicSmemBytes = fixed + (q.p.E + 1) * 8;
+    c.dynamicSmemBytes = fixed + groups_bytes(q.p.E);
     c.stream = s;
     cudaLaunchAttribute attr[2];
     c.attrs = attr;
@@ -1780,11 +1770,14 @@ cudaError_t run_stream(const LinParams &p, bool bf, cudaStream_t s) {
     q.vec_x = (uintptr_t)p.x % 16 == 0 && (p.M == 1 || p.ldx % 8 == 0);
     const uint64_t row_tiles = p.E == 1 ? (p.M + (two ? 15 : 7)) / (two ? 16 : 8)
                                         : p.M / (two ? 16 : 8) + active;
-    const uint64_t tiles = row_tiles * ((p.N + 127) / 128);
+    q.tile = Divisor(two ? 16 : 8);
+    q.nt = Divisor((p.N + 127) / 128);
+    const uint64_t tiles = row_tiles * q.nt.d;
     if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
     // two CTAs fit an SM; a part keeps at least a block for each warp
     q.split = 1;
     while (q.split < 8 && tiles * q.split * 2 <= 2 * sms && kbs >= q.split * 2 * ST_WARPS) q.split *= 2;
+    while (1u << q.shift < q.split) q.shift++;
     const uint32_t grid = (uint32_t)tiles * q.split;
     if (bf) return two ? launch_stream<true, 2>(q, grid, s) : launch_stream<true, 1>(q, grid, s);
     return two ? launch_stream<false, 2>(q, grid, s) : launch_stream<false, 1>(q, grid, s);
@@ -1824,20 +1817,15 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     p.vec_res = rows16(p.res, p.ldres, osz);
     p.vec_out = rows16(p.out, p.ldo, osz);
     const bool bf = a->x_dtype == HCT_B200_BF16, int4 = a->weight_form == HCT_B200_WEIGHT_INT4;
-    if (int4 && p.M <= STREAM_ROWS * std::min(p.E, p.M)) return code_of(run_stream(p, bf, s));
-    // the tensor cores take rows that TMA can fetch (and strides that its maps can hold)
-    const bool w_ok = int4 || (tma_rows(p.w, p.N, p.ldw, p.K) &&
-                               (p.E == 1 || (p.w_stride % 8 == 0 && p.w_stride && p.w_stride < 1ull << 38)));
-    if (p.K && w_ok && tma_rows(p.x, p.M, p.ldx, p.K)) return code_of(run_umma(p, grouped, int4, bf, s));
-    // at most this many row tiles: one partial tile per expert beside the whole ones
-    const uint64_t mt = p.M / SM_M + std::min<uint64_t>(p.E, p.M);
-    const uint64_t tiles = mt * ((p.N + SM_N - 1) / SM_N);
-    const unsigned grid = (unsigned)std::min<uint64_t>(tiles, 8ull * sm_count());
-    if (bf && int4) linear_plain_kernel<true, true><<<grid, SM_THREADS, 0, s>>>(p);
-    else if (bf) linear_plain_kernel<true, false><<<grid, SM_THREADS, 0, s>>>(p);
-    else if (int4) linear_plain_kernel<false, true><<<grid, SM_THREADS, 0, s>>>(p);
-    else linear_plain_kernel<false, false><<<grid, SM_THREADS, 0, s>>>(p);
-    return code_of(cudaGetLastError());
+    const bool x_rows = tma_rows(p.x, p.M, p.ldx, p.K);
+    if (int4) {
+        // the stream kernel for a few rows, and for any number of rows that TMA cannot fetch
+        if (!x_rows || p.M <= STREAM_ROWS * std::min(p.E, p.M)) return code_of(run_stream(p, bf, s));
+        return code_of(run_umma(p, grouped, FORM_INT4, bf, s));
+    }
+    const bool w_rows = tma_rows(p.w, p.N, p.ldw, p.K) &&
+                        (p.E == 1 || (p.w_stride % 8 == 0 && p.w_stride && p.w_stride < 1ull << 38));
+    return code_of(run_umma(p, grouped, p.K && x_rows && w_rows ? FORM_DENSE : FORM_ANY, bf, s));
 }
 
 }  // namespace
