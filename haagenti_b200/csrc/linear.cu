@@ -97,7 +97,8 @@ struct Divisor {
 struct LinParams {
     const void *x, *w, *bias, *gate, *res, *offsets;
     void *out;
-    uint64_t ldx, ldw, w_stride, ldgate, ldres, ldo;
+    uint64_t w_stride;
+    uint32_t ldx, ldw, ldgate, ldres, ldo;  // at most 2^30
     uint32_t M, N, K, E;
     int off64;  // offsets are int64 (else int32)
     int bias_f32, act, odt;
@@ -190,14 +191,28 @@ __device__ __forceinline__ float from16(uint16_t v) {
     return BF ? bf2f(v) : h2f(v);
 }
 
+template <class T>
+__device__ __forceinline__ uint32_t bits_of(T v) {
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+
+// z / (1 + 2^(-t log2 e)): the hardware's ex2 and reciprocal, a few 2^-23 of the
+// value, as the rest of the f32 epilogue.
+__device__ __forceinline__ float times_sigmoid(float z, float minus_t_log2e) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(minus_t_log2e));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return z * r;
+}
 __device__ __forceinline__ float activate(float z, int act) {
+    constexpr float LOG2E = 1.44269504088896341f;
     switch (act) {
         case HCT_B200_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        // __expf and __fdividef: a few 2^-23 of the value, as the rest of the f32 epilogue
-        case HCT_B200_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
+        case HCT_B200_ACT_SILU: return times_sigmoid(z, -LOG2E * z);
         case HCT_B200_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
         case HCT_B200_ACT_GELU_TANH:  // (1 + tanh(t)) / 2 = 1 / (1 + e^-2t)
-            return __fdividef(z, 1.0f + __expf(-1.59576912160573071f * (z + 0.044715f * z * z * z)));
+            return times_sigmoid(
+                z, z * fmaf(-0.0713548162726f * LOG2E, z * z, -1.59576912160573071f * LOG2E));
         default: return z;
     }
 }
@@ -500,6 +515,13 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
+// The last barrier of a cluster: no CTA ends while another may still read its
+// memory.  Nothing is published, so the arrival need not wait for the outputs'
+// stores.
+__device__ __forceinline__ void cluster_leave() {
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+}
 __device__ __forceinline__ float4 ld_cluster(uint32_t saddr, uint32_t rank) {
     uint32_t a;
     float4 v;
@@ -564,10 +586,6 @@ struct Scale<true> {
         lo = __bfloat162bfloat162(__float2bfloat16_rn(finite ? f - __bfloat162float(h) : 0.0f));
     }
 };
-template <class T>
-__device__ __forceinline__ uint32_t bits_of(T v) {
-    return *reinterpret_cast<uint32_t *>(&v);
-}
 template <bool PRECISE>
 __device__ __forceinline__ void dequant8(uint32_t w, const Scale<false> &s, uint32_t (&v)[4],
                                          uint32_t (&l)[4]) {
@@ -605,65 +623,69 @@ __device__ __forceinline__ void activate_all(float (&z)[W]) {
     for (int j = 0; j < W; j++) z[j] = activate(z[j], ACT);
 }
 
-// The operands of 8 consecutive features n .. n + 7 of row m: gate in g, the
-// residual in r (8 16-bit values in r[0..3], or 8 floats).  Whole 16-byte
-// pieces where the row allows them, else element by element.
+// What an epilogue writes: F32, one of the 16-bit types, or any.
+enum { OUT_F32 = 0, OUT_16 = 1, OUT_ANY = 2 };
+template <int OUT>
+__device__ __forceinline__ bool writes_f32(const LinParams &p) {
+    return OUT == OUT_F32 || (OUT == OUT_ANY && p.odt == HCT_B200_F32);
+}
+
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+    if (BF) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+
+// 8 consecutive 16-bit values, `live` of which exist; one load where aligned.
+__device__ __forceinline__ void load8(const uint16_t *q, bool vec, uint32_t live, uint32_t (&v)[4]) {
+    if (vec && live >= 8) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(q);
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = 2 * j < (int)live ? q[2 * j] : 0u;
+            if (2 * j + 1 < (int)live) v[j] |= (uint32_t)q[2 * j + 1] << 16;
+        }
+    }
+}
+
+// The operands of 8 consecutive features n .. n + 7 of row m: the gate in g, the
+// residual in r (8 16-bit values in r[0..3], or 8 floats).
 struct Operands {
     uint32_t g[4], r[8];
 };
-template <int ODT>
+template <int OUT>
 __device__ __forceinline__ void load_operands(const LinParams &p, uint32_t m, uint32_t n,
                                               Operands &o) {
-    const bool whole = n + 8 <= p.N;
-    if (p.gate) {
-        const uint16_t *q = reinterpret_cast<const uint16_t *>(p.gate) + (uint64_t)m * p.ldgate + n;
-        if (whole && p.vec_gate) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(q);
-            o.g[0] = v.x, o.g[1] = v.y, o.g[2] = v.z, o.g[3] = v.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                o.g[j] = (n + 2 * j < p.N ? q[2 * j] : 0u) |
-                         (n + 2 * j + 1 < p.N ? (uint32_t)q[2 * j + 1] << 16 : 0u);
-        }
-    }
+    const uint32_t live = p.N - n;
+    if (p.gate)
+        load8(reinterpret_cast<const uint16_t *>(p.gate) + (uint64_t)m * p.ldgate + n, p.vec_gate, live,
+              o.g);
     if (p.res) {
         const uint64_t at = (uint64_t)m * p.ldres + n;
-        if (ODT == HCT_B200_F32) {
+        if (writes_f32<OUT>(p)) {
             const uint32_t *q = reinterpret_cast<const uint32_t *>(p.res) + at;
-            if (whole && p.vec_res) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint4 v = reinterpret_cast<const uint4 *>(q)[h];
-                    o.r[4 * h] = v.x, o.r[4 * h + 1] = v.y, o.r[4 * h + 2] = v.z, o.r[4 * h + 3] = v.w;
-                }
+            if (p.vec_res && live >= 8) {
+                const uint4 a = reinterpret_cast<const uint4 *>(q)[0];
+                const uint4 b = reinterpret_cast<const uint4 *>(q)[1];
+                o.r[0] = a.x, o.r[1] = a.y, o.r[2] = a.z, o.r[3] = a.w;
+                o.r[4] = b.x, o.r[5] = b.y, o.r[6] = b.z, o.r[7] = b.w;
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) o.r[j] = n + j < p.N ? q[j] : 0u;
+                for (int j = 0; j < 8; j++) o.r[j] = j < (int)live ? q[j] : 0u;
             }
         } else {
-            const uint16_t *q = reinterpret_cast<const uint16_t *>(p.res) + at;
-            if (whole && p.vec_res) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(q);
-                o.r[0] = v.x, o.r[1] = v.y, o.r[2] = v.z, o.r[3] = v.w;
-            } else {
+            uint32_t v[4];
+            load8(reinterpret_cast<const uint16_t *>(p.res) + at, p.vec_res, live, v);
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    o.r[j] = (n + 2 * j < p.N ? q[2 * j] : 0u) |
-                             (n + 2 * j + 1 < p.N ? (uint32_t)q[2 * j + 1] << 16 : 0u);
-            }
+            for (int j = 0; j < 4; j++) o.r[j] = v[j];
         }
     }
-}
-
-template <int ODT>
-__device__ __forceinline__ uint32_t to16(float v) {
-    return ODT == HCT_B200_F16 ? (uint32_t)__half_as_ushort(__float2half_rn(v))
-                               : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
 // 8 sums (bias included) of row m, features n .. n + 7, to outputs.
-template <bool BF, int ODT>
+template <bool BF, int OUT>
 __device__ __forceinline__ void finish8(const LinParams &p, float (&z)[8], const Operands &o,
                                         uint32_t m, uint32_t n) {
     switch (p.act) {
@@ -675,18 +697,19 @@ __device__ __forceinline__ void finish8(const LinParams &p, float (&z)[8], const
     }
     if (p.gate) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) z[j] *= from16<BF>((uint16_t)(o.g[j / 2] >> (16 * (j & 1))));
+        for (int j = 0; j < 4; j++) {
+            const float2 g = unpack2<BF>(o.g[j]);
+            z[2 * j] *= g.x, z[2 * j + 1] *= g.y;
+        }
     }
-    if (p.res) {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            z[j] += ODT == HCT_B200_F32
-                        ? __uint_as_float(o.r[j])
-                        : from16<ODT == HCT_B200_BF16>((uint16_t)(o.r[j / 2] >> (16 * (j & 1))));
-    }
+    const uint32_t live = p.N - n;
+    const bool whole = p.vec_out && live >= 8;
     const uint64_t at = (uint64_t)m * p.ldo + n;
-    const bool whole = n + 8 <= p.N && p.vec_out;
-    if (ODT == HCT_B200_F32) {
+    if (writes_f32<OUT>(p)) {
+        if (p.res) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) z[j] += __uint_as_float(o.r[j]);
+        }
         float *q = reinterpret_cast<float *>(p.out) + at;
         if (whole) {
             reinterpret_cast<float4 *>(q)[0] = make_float4(z[0], z[1], z[2], z[3]);
@@ -694,34 +717,42 @@ __device__ __forceinline__ void finish8(const LinParams &p, float (&z)[8], const
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (n + j < p.N) q[j] = z[j];
+                if (j < (int)live) q[j] = z[j];
         }
     } else {
-        uint16_t *q = reinterpret_cast<uint16_t *>(p.out) + at;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = to16<ODT>(z[2 * j]) | to16<ODT>(z[2 * j + 1]) << 16;
+        for (int j = 0; j < 4; j++) {
+            float a = z[2 * j], b = z[2 * j + 1];
+            if (p.odt == HCT_B200_F16) {
+                if (p.res) {
+                    const float2 r = unpack2<false>(o.r[j]);
+                    a += r.x, b += r.y;
+                }
+                w[j] = bits_of(__floats2half2_rn(a, b));
+            } else {
+                if (p.res) {
+                    const float2 r = unpack2<true>(o.r[j]);
+                    a += r.x, b += r.y;
+                }
+                w[j] = bits_of(__floats2bfloat162_rn(a, b));
+            }
+        }
+        uint16_t *q = reinterpret_cast<uint16_t *>(p.out) + at;
         if (whole) {
             *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (n + j < p.N) q[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+                if (j < (int)live) q[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
         }
     }
-}
-template <bool BF, bool PRECISE>
-__device__ __forceinline__ void finish8_any(const LinParams &p, float (&z)[8], const Operands &o,
-                                            uint32_t m, uint32_t n) {
-    if (PRECISE) finish8<BF, HCT_B200_F32>(p, z, o, m, n);
-    else if (p.odt == HCT_B200_F16) finish8<BF, HCT_B200_F16>(p, z, o, m, n);
-    else finish8<BF, HCT_B200_BF16>(p, z, o, m, n);
 }
 
 // Sixteen rows m .. m + 15 (count of them live) of a tile's 128 features, a
 // feature per thread of the set in z: through the set's shared memory (16 x
 // 128 floats) to its threads by rows, each 2 rows x 8 features n .. n + 7.
-template <bool BF, bool PRECISE>
+template <bool BF, int OUT>
 __device__ __forceinline__ void finish_rows(const LinParams &p, const float (&z)[16], float *stage,
                                             uint32_t set, uint32_t id, const float (&bias)[8],
                                             uint32_t m, uint32_t count, uint32_t n) {
@@ -730,7 +761,7 @@ __device__ __forceinline__ void finish_rows(const LinParams &p, const float (&z)
     const bool live = n < p.N;
 #pragma unroll
     for (int i = 0; i < 2; i++)
-        if (live && j0 + 8 * i < count) load_operands<PRECISE ? HCT_B200_F32 : HCT_B200_F16>(p, m + j0 + 8 * i, n, o[i]);
+        if (live && j0 + 8 * i < count) load_operands<OUT>(p, m + j0 + 8 * i, n, o[i]);
     asm volatile("bar.sync %0, 128;" ::"r"(set + 1) : "memory");  // the last rows have been read
 #pragma unroll
     for (int j = 0; j < 16; j++) stage[j * 128 + id] = z[j];
@@ -742,7 +773,7 @@ __device__ __forceinline__ void finish_rows(const LinParams &p, const float (&z)
         const float4 a = q[0], b = q[1];
         float v[8] = {a.x + bias[0], a.y + bias[1], a.z + bias[2], a.w + bias[3],
                       b.x + bias[4], b.y + bias[5], b.z + bias[6], b.w + bias[7]};
-        finish8_any<BF, PRECISE>(p, v, o[i], m + j0 + 8 * i, n);
+        finish8<BF, OUT>(p, v, o[i], m + j0 + 8 * i, n);
     }
 }
 
@@ -780,24 +811,26 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
     const Groups groups(reinterpret_cast<uint32_t *>(ctl + 1), p.E);
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
 
-    if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < stages; s++) {
-            mbar_init(smem_u32(&ctl->xfull[s]), 1);
-            mbar_init(smem_u32(&ctl->afull[s]), 4 * CTAS);
-            mbar_init(smem_u32(&ctl->empty[s]), 1);
+    if (warp == 0) {
+        if (lane < MAX_STAGES) {
+            mbar_init(smem_u32(&ctl->xfull[lane]), 1);
+            mbar_init(smem_u32(&ctl->afull[lane]), 4 * CTAS);
+            mbar_init(smem_u32(&ctl->empty[lane]), 1);
         }
-        for (uint32_t s = 0; s < u.raw_stages; s++) {
-            mbar_init(smem_u32(&ctl->rfull[s]), 1);
-            mbar_init(smem_u32(&ctl->rempty[s]), 4);
+        if (INT4 && lane < MAX_RAW) {
+            mbar_init(smem_u32(&ctl->rfull[lane]), 1);
+            mbar_init(smem_u32(&ctl->rempty[lane]), 4);
         }
-        for (int b = 0; b < 2; b++) {
-            mbar_init(smem_u32(&ctl->tfull[b]), 1);
-            mbar_init(smem_u32(&ctl->tempty[b]), 8 * CTAS);
+        if (lane < 2) {
+            mbar_init(smem_u32(&ctl->tfull[lane]), 1);
+            mbar_init(smem_u32(&ctl->tempty[lane]), 8 * CTAS);
         }
-        mbar_init(smem_u32(&ctl->drain), 1);
-        ctl->abort = 0;
-        ctl->issued = 0;
-        ctl->raw_issued = 0;
+        if (lane == 0) {
+            mbar_init(smem_u32(&ctl->drain), 1);
+            ctl->abort = 0;
+            ctl->issued = 0;
+            ctl->raw_issued = 0;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -1075,7 +1108,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
 #pragma unroll
                             for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + id] = z[j];
                         } else {
-                            finish_rows<BF, false>(p, z, stage, set, id, bias, c.m0 + j0,
+                            finish_rows<BF, OUT_16>(p, z, stage, set, id, bias, c.m0 + j0,
                                                    c.rows - j0, n);
                         }
                     }
@@ -1097,7 +1130,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
 #pragma unroll
                         for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + id] = sum[i][j];
                     } else {
-                        finish_rows<BF, true>(p, sum[i], stage, set, id, bias, c.m0 + j0, c.rows - j0, n);
+                        finish_rows<BF, OUT_F32>(p, sum[i], stage, set, id, bias, c.m0 + j0, c.rows - j0, n);
                     }
                 }
             }
@@ -1109,42 +1142,51 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         // one tile per cluster: each CTA finishes its share of the tile's rows,
         // adding the CTAs' parts in rank order.  Both barriers are reached by
         // every thread of every CTA on every path.
-        __syncwarp();
-        cluster_barrier();
-        if (t0 < tiles && !aborted()) {
-            const Tile c = tile_at<FEATURES>(u, groups, t0);
-            const uint32_t j0 = c.rows * rank / u.split, j1 = c.rows * (rank + 1) / u.split;
-            const uint32_t f = threadIdx.x % 16 * 8, n = c.n0 + f, base = smem_u32(smem);
-            if (n < p.N) {
-                float bias[8];
+        constexpr int OUT = PRECISE ? OUT_F32 : OUT_16;
+        Tile c{};
+        uint32_t j = 0, j1 = 0, n = 0;
+        float bias[8];
+        Operands o;
+        if (t0 < tiles) {
+            c = tile_at<FEATURES>(u, groups, t0);
+            n = c.n0 + threadIdx.x % 16 * 8;
+            j1 = n < p.N ? c.rows * (rank + 1) / u.split : 0;
+            j = c.rows * rank / u.split + threadIdx.x / 16;
+            if (j < j1) {
                 load_bias8<BF>(p, c.e, n, bias);
-                for (uint32_t j = j0 + threadIdx.x / 16; j < j1; j += blockDim.x / 16) {
-                    Operands o;
-                    load_operands<PRECISE ? HCT_B200_F32 : HCT_B200_F16>(p, c.m0 + j, n, o);
-                    float z[8] = {};
-#pragma unroll
-                    for (uint32_t r0 = 0; r0 < 8; r0 += 4) {  // four parts in flight
-                        float4 a[4], b[4];
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; i++)
-                            if (r0 + i < u.split) {
-                                a[i] = ld_cluster(base + (j * 128 + f) * 4, r0 + i);
-                                b[i] = ld_cluster(base + (j * 128 + f + 4) * 4, r0 + i);
-                            }
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; i++)
-                            if (r0 + i < u.split) {
-                                z[0] += a[i].x, z[1] += a[i].y, z[2] += a[i].z, z[3] += a[i].w;
-                                z[4] += b[i].x, z[5] += b[i].y, z[6] += b[i].z, z[7] += b[i].w;
-                            }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; i++) z[i] += bias[i];
-                    finish8_any<BF, PRECISE>(p, z, o, c.m0 + j, n);
-                }
+                load_operands<OUT>(p, c.m0 + j, n, o);
             }
         }
+        __syncwarp();
         cluster_barrier();
+        if (!aborted()) {
+            const uint32_t f = threadIdx.x % 16 * 8, base = smem_u32(smem);
+            while (j < j1) {
+                float z[8] = {};
+#pragma unroll
+                for (uint32_t r0 = 0; r0 < 8; r0 += 4) {  // four parts in flight
+                    float4 a[4], b[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++)
+                        if (r0 + i < u.split) {
+                            a[i] = ld_cluster(base + (j * 128 + f) * 4, r0 + i);
+                            b[i] = ld_cluster(base + (j * 128 + f + 4) * 4, r0 + i);
+                        }
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++)
+                        if (r0 + i < u.split) {
+                            z[0] += a[i].x, z[1] += a[i].y, z[2] += a[i].z, z[3] += a[i].w;
+                            z[4] += b[i].x, z[5] += b[i].y, z[6] += b[i].z, z[7] += b[i].w;
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) z[i] += bias[i];
+                finish8<BF, OUT>(p, z, o, c.m0 + j, n);
+                j += blockDim.x / 16;
+                if (j < j1) load_operands<OUT>(p, c.m0 + j, n, o);
+            }
+        }
+        cluster_leave();
     }
 
     // ---- teardown: nothing of this CTA may be in flight when it ends --------------
@@ -1164,7 +1206,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         if (!mbar_wait(smem_u32(&ctl->drain), 0, &go_on)) give_up();
     }
     __syncthreads();
-    if (PAIR) cluster_barrier();  // neither CTA's memory is in use any more
+    if (PAIR) cluster_leave();  // neither CTA's memory is in use any more
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         tmem_free<PAIR>(tmem, u.tmem_cols);
@@ -1415,28 +1457,25 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
             z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
         }
     }
-    const auto finish = [&](uint32_t r) {
-        if (n >= p.N) return;
-        Operands o;
-        const uint32_t m = m0 + r;
-        float bias[8];
+    // what the rows that this thread finishes need beside their sums
+    const uint32_t mine = (row << q.shift) + rank;  // of a split: row r is finished by CTA r % split
+    const bool mine_live = mine < rows && n < p.N;
+    float bias[8];
+    Operands o;
+    if (mine_live) {
         load_bias8<BF>(p, e, n, bias);
+        load_operands<OUT_ANY>(p, m0 + mine, n, o);
+    }
+    const auto finish = [&]() {
 #pragma unroll
         for (int j = 0; j < 8; j++) z[j] += bias[j];
-        if (p.odt == HCT_B200_F32) {
-            load_operands<HCT_B200_F32>(p, m, n, o);
-            finish8<BF, HCT_B200_F32>(p, z, o, m, n);
-        } else {
-            load_operands<HCT_B200_F16>(p, m, n, o);
-            finish8_any<BF, false>(p, z, o, m, n);
-        }
+        finish8<BF, OUT_ANY>(p, z, o, m0 + mine, n);
     };
     if (q.split == 1) {
-        if (row < rows) finish(row);
+        if (mine_live) finish();
         return;
     }
-    // row r is finished by CTA r % split, which receives its parts at
-    // [r / split][source rank]
+    // CTA r % split receives the parts of row r at [r / split][source rank]
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (row < rows) {
         const uint32_t at = smem_u32(recv + ((row >> q.shift << q.shift) + rank) * 128 + f);
@@ -1449,8 +1488,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
                      : "memory");
     }
     cluster_barrier();
-    const uint32_t mine = (row << q.shift) + rank;  // this thread's row, of those that I finish
-    if (mine < rows) {
+    if (mine_live) {
 #pragma unroll
         for (int j = 0; j < 8; j++) z[j] = 0.0f;
 #pragma unroll
@@ -1461,7 +1499,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
             z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
             z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
         }
-        finish(mine);
+        finish();
     }
 }
 
@@ -1680,13 +1718,13 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     UmmaParams u{};
     u.p = p;
     u.split = 1;
-    // pairs where tiles of 256 features and full height keep every pair busy
-    const bool pair = !precise && !any && per_expert >= 192 &&
-                      (uint64_t)((p.N + 255) / 256) * (p.M / 256) * 2 >= sms;
+    // pairs where tiles of 256 features keep every pair busy
+    const uint64_t pair_tiles = (uint64_t)((p.N + 255) / 256) * ((p.M + 255) / 256 + (active - 1) / 2);
+    const bool pair = !precise && !any && per_expert > 64 && pair_tiles * 2 >= sms;
     const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128, units = pair ? sms / 2 : sms;
     uint64_t row_tiles;  // at most
     if (grouped) {
-        u.bn = std::min(cap, per_expert <= 64 ? 128u : 256u);
+        u.bn = std::min(cap, pair || per_expert > 64 ? 256u : 128u);
         u.xbox = 32;
         row_tiles = p.M / u.bn + active;
     } else {
@@ -1795,12 +1833,12 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     p.res = a->d_residual;
     p.offsets = grouped ? a->d_offsets : nullptr;
     p.out = a->d_out;
-    p.ldx = a->ldx;
-    p.ldw = a->ldw;
+    p.ldx = (uint32_t)a->ldx;
+    p.ldw = (uint32_t)a->ldw;
     p.w_stride = a->weight_stride;
-    p.ldgate = a->ldgate;
-    p.ldres = a->ldresidual;
-    p.ldo = a->ldout;
+    p.ldgate = (uint32_t)a->ldgate;
+    p.ldres = (uint32_t)a->ldresidual;
+    p.ldo = (uint32_t)a->ldout;
     p.M = (uint32_t)a->rows;
     p.N = (uint32_t)a->out_features;
     p.K = (uint32_t)a->in_features;
