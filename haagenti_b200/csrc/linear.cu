@@ -238,7 +238,11 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 //
 //   warp 0      TMA producer: x tiles (and dense weight tiles) into a ring of
 //               K steps of 64, packed INT4 blocks into a ring of their own
-//   warp 1      TMEM allocation; one thread issues the MMAs
+//   warp 1      TMEM allocation; one thread issues the MMAs.  Up to 128 rows the
+//               issuing (450 to 600 clocks a K step: a wait, four MMAs, a commit)
+//               takes longer than the MMAs (256), so warps 1 and 2 issue every
+//               other K step each (the even and the odd slots of the ring), into
+//               accumulators of their own
 //   warps 4-11  epilogue, two sets of four warps that take every other 16 rows:
 //               accumulators (TMEM lanes = features) through shared memory into
 //               runs of 8 features, so that outputs, gate and residual move in
@@ -263,6 +267,14 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 // sections in registers with rounding; INT4 weights are then two A operands,
 // the rounded weight and what the rounding left.
 //
+// A wait on a slot's parity is sound only for one that cannot be two passes
+// behind.  The producers and issuers meet every pass of a slot in order.  The
+// three dequantising or loading groups take the steps of a slot by turns: the
+// packed ring has a multiple of 3 slots, so that a slot is always one group's;
+// a slot of the operand ring is one group's too where there are two issuers (6
+// slots), and with one issuer, whose MMAs complete in order, the step before
+// in the group has already seen every step up to its own less (slots + 3).
+//
 // Every wait is bounded; an expired one raises g_linear_status, the CTA's
 // roles leave their loops, its copies and MMAs are drained (bounded) and TMEM
 // is freed.
@@ -282,6 +294,7 @@ struct UmmaParams {
     uint32_t stages, raw_stages;
     uint32_t tmem_cols, tmem_stride;
     uint32_t split;   // CTAs per cluster, each a part of K
+    uint32_t issuers; // warps that issue MMAs, each with its own accumulators
     Divisor tile, nt, band;  // by bn, by feature tiles, by RASTER x feature tiles
 };
 
@@ -822,11 +835,11 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
             mbar_init(smem_u32(&ctl->rempty[lane]), 4);
         }
         if (lane < 2) {
-            mbar_init(smem_u32(&ctl->tfull[lane]), 1);
+            mbar_init(smem_u32(&ctl->tfull[lane]), u.issuers);
             mbar_init(smem_u32(&ctl->tempty[lane]), 8 * CTAS);
         }
         if (lane == 0) {
-            mbar_init(smem_u32(&ctl->drain), 1);
+            mbar_init(smem_u32(&ctl->drain), u.issuers);
             ctl->abort = 0;
             ctl->issued = 0;
             ctl->raw_issued = 0;
@@ -862,7 +875,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         kb0 = kbs * rank / u.split;
         kb1 = kbs * (rank + 1) / u.split;
     }
-    const uint32_t sect = PRECISE ? SECTION : kb1 - kb0;  // K steps per accumulation
+    const uint32_t sect = PRECISE ? SECTION * u.issuers : kb1 - kb0;  // K steps per accumulation
 
     // The producers and the MMA warp run whole (their addresses and descriptors
     // are warp-uniform); one elected lane issues.
@@ -898,24 +911,27 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         }
         if (lane == 0) ctl->issued = (int)issued;
         if (!ok) give_up();
-    } else if (warp == 1) {
+    } else if (warp == 1 || (warp == 2 && u.issuers == 2)) {
         // D = F32, A = B = x's type, both K-major, M = FEATURES; N follows the tile
         const uint32_t idesc0 =
             (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((FEATURES / 16) << 24);
         // INT4: half of the lanes wait for the x tile, half for the weights
         const uint32_t full = smem_u32(ANY || (INT4 && lane >= 16) ? ctl->afull : ctl->xfull);
+        const uint32_t me = warp - 1, every = u.issuers - 1;  // slots: me modulo u.issuers
         Ring at(stages), acc(2);
         bool ok = true;
         for (uint32_t t = t0; side == 0 && ok && t < tiles; t += step) {
             const Tile c = tile_at<FEATURES>(u, groups, t);
             const uint32_t idesc = uniform(idesc0 | ((c.rows + 15) / 16 * 2) << 17);
             for (uint32_t kb = kb0; ok && kb < kb1; acc.step()) {
-                const uint32_t end = min(kb + sect, kb1), from = kb;
+                const uint32_t end = min(kb + sect, kb1);
+                bool fresh = true;  // nothing accumulated yet
                 ok = mbar_wait_warp(smem_u32(&ctl->tempty[acc.slot]), acc.pass ^ 1u, &ctl->abort);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + acc.slot * u.tmem_stride;
+                const uint32_t d = tmem + (acc.slot * u.issuers + me) * u.tmem_stride;
                 for (; kb < end; kb++, at.step()) {
+                    if ((at.slot & every) != me) continue;
                     ok = mbar_wait_warp(full + at.slot * 8, at.pass, &ctl->abort);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -927,10 +943,11 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
 #pragma unroll
                             for (uint32_t k = 0; k < BK / 16; k++)
                                 umma<PAIR>(d, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k, idesc,
-                                           kb != from || a || k);
+                                           !fresh || a || k);
                         umma_commit<PAIR>(smem_u32(&ctl->empty[at.slot]));
                     }
                     __syncwarp();
+                    fresh = false;
                 }
                 if (ok && elect_one()) umma_commit<PAIR>(smem_u32(&ctl->tfull[acc.slot]));
                 __syncwarp();
@@ -1066,6 +1083,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         float *part = reinterpret_cast<float *>(smem);  // split: [rows of x][128 features]
         float *stage = reinterpret_cast<float *>(epi + set * (EPI_BYTES / 2));
         Ring acc(2);
+        uint32_t steps = 0;  // K steps of the sections before
         bool ok = true;
         for (uint32_t t = t0; ok && t < tiles; t += step) {
             const Tile c = tile_at<FEATURES>(u, groups, t);
@@ -1084,7 +1102,12 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                 if (!PRECISE) ok = set_agrees(set, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t ta = tmem + acc.slot * u.tmem_stride + ((q * 32) << 16);
+                // a section of one K step is in the accumulators of that step's issuer
+                const bool two = u.issuers == 2 && kb + 1 < kb1;
+                const uint32_t lone = two ? 0 : steps & (u.issuers - 1);
+                const uint32_t ta =
+                    tmem + (acc.slot * u.issuers + lone) * u.tmem_stride + ((q * 32) << 16);
+                steps += min(sect, kb1 - kb);
                 if (PRECISE) {
 #pragma unroll
                     for (int i = 0; i < (PRECISE ? CHUNKS : 1); i++) {
@@ -1095,6 +1118,11 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                         tmem_ld16(ta + j0, v);
 #pragma unroll
                         for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
+                        if (two) {
+                            tmem_ld16(ta + u.tmem_stride + j0, v);
+#pragma unroll
+                            for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
+                        }
                     }
                 } else {
                     for (uint32_t j0 = set * 16; j0 < c.rows; j0 += 32) {
@@ -1104,6 +1132,11 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                         tmem_ld16(ta + j0, v);
 #pragma unroll
                         for (int j = 0; j < 16; j++) z[j] = __uint_as_float(v[j]);
+                        if (two) {
+                            tmem_ld16(ta + u.tmem_stride + j0, v);
+#pragma unroll
+                            for (int j = 0; j < 16; j++) z[j] += __uint_as_float(v[j]);
+                        }
                         if (u.split > 1) {
 #pragma unroll
                             for (int j = 0; j < 16; j++) part[(j0 + j) * 128 + id] = z[j];
@@ -1743,16 +1776,24 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
         grid = u.split > 1 ? (uint32_t)tiles * u.split : (uint32_t)std::min<uint64_t>(tiles, sms);
     }
     u.tmem_stride = round_to(u.bn, 32);
-    u.tmem_cols = 64;
-    while (u.tmem_cols < 2 * u.tmem_stride) u.tmem_cols *= 2;
+    // two issuers where their accumulators fit TMEM twice and an operand ring of 6
+    // slots (any even number without groups) fits shared memory
     const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn / (pair ? 2 : 1) * 128;
-    u.raw_stages = int4 ? 10 : 0;
-    const uint32_t fixed =
-        1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) + groups_bytes(p.E);
+    u.issuers = u.bn <= (int4 ? 96u : 128u) && !(int4 && precise) ? 2 : 1;
+    u.raw_stages = !int4 ? 0 : u.issuers == 2 && u.bn > 64 ? 6 : 9;
+    const uint32_t fixed = 1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) +
+                           groups_bytes(p.E);
+    u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
+    if (u.issuers == 2) {
+        if (form == FORM_DENSE) u.stages &= ~1u;
+        else if (u.stages >= 6) u.stages = 6;
+        else u.issuers = 1;  // many experts' tables
+    }
+    u.tmem_cols = 64;
+    while (u.tmem_cols < 2 * u.issuers * u.tmem_stride) u.tmem_cols *= 2;
     u.tile = Divisor(u.bn);
     u.nt = Divisor(nt);
     u.band = Divisor(nt * RASTER);
-    u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
     const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
 
     alignas(64) CUtensorMap tx{}, tw{};
