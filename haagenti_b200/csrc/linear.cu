@@ -915,8 +915,14 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         // D = F32, A = B = x's type, both K-major, M = FEATURES; N follows the tile
         const uint32_t idesc0 =
             (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((FEATURES / 16) << 24);
-        // INT4: half of the lanes wait for the x tile, half for the weights
-        const uint32_t full = smem_u32(ANY || (INT4 && lane >= 16) ? ctl->afull : ctl->xfull);
+        // INT4: half of the lanes wait for the x tile, half for the weights; the upper
+        // half of the warp for the second of two K steps
+        const uint32_t full = smem_u32(ANY || (INT4 && (lane & 8u)) ? ctl->afull : ctl->xfull);
+        // INT4: two steps to a wait where that leaves the ring three to be filled
+        // meanwhile.  The issuing warp shares its scheduler with three dequantising
+        // ones; 2048 x 14336 x 4096 takes 192 us for 203.  Dense operands, which come
+        // in order from one producer, lose by it (170 us for 168)
+        const bool pairs = INT4 && u.issuers == 1 && stages >= 5;
         const uint32_t me = warp - 1, every = u.issuers - 1;  // slots: me modulo u.issuers
         Ring at(stages), acc(2);
         bool ok = true;
@@ -930,24 +936,37 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + (acc.slot * u.issuers + me) * u.tmem_stride;
-                for (; kb < end; kb++, at.step()) {
-                    if ((at.slot & every) != me) continue;
-                    ok = mbar_wait_warp(full + at.slot * 8, at.pass, &ctl->abort);
+                while (kb < end) {
+                    if ((at.slot & every) != me) {
+                        kb++, at.step();
+                        continue;
+                    }
+                    const Ring here = at;
+                    const bool two = pairs && kb + 1 < end;
+                    kb++, at.step();
+                    const bool later = two && lane >= 16;
+                    ok = mbar_wait_warp(full + (later ? at.slot : here.slot) * 8,
+                                        later ? at.pass : here.pass, &ctl->abort);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t sa = smem_u32(smem) + at.slot * stage_bytes;
-                    const uint64_t da = umma_desc(sa), db = umma_desc(sa + A_PARTS * A_BYTES);
-                    if (elect_one()) {
+                    const auto issue = [&](uint32_t slot, bool more) {
+                        const uint32_t sa = smem_u32(smem) + slot * stage_bytes;
+                        const uint64_t da = umma_desc(sa), db = umma_desc(sa + A_PARTS * A_BYTES);
 #pragma unroll
                         for (uint32_t a = 0; a < A_PARTS; a++)
 #pragma unroll
                             for (uint32_t k = 0; k < BK / 16; k++)
                                 umma<PAIR>(d, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k, idesc,
-                                           !fresh || a || k);
-                        umma_commit<PAIR>(smem_u32(&ctl->empty[at.slot]));
+                                           more || a || k);
+                        umma_commit<PAIR>(smem_u32(&ctl->empty[slot]));
+                    };
+                    if (elect_one()) {
+                        issue(here.slot, !fresh);
+                        if (two) issue(at.slot, true);
                     }
                     __syncwarp();
                     fresh = false;
+                    if (two) kb++, at.step();
                 }
                 if (ok && elect_one()) umma_commit<PAIR>(smem_u32(&ctl->tfull[acc.slot]));
                 __syncwarp();
@@ -1051,20 +1070,23 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                 const uint32_t k = kb * BK + col;
                 const auto copy = [&](const uint16_t *src, uint64_t ld, uint32_t row0, uint32_t live,
                                       uint32_t r0, uint32_t count, uint8_t *dst) {
-                    for (uint32_t i = 0; i < count; i += 4) {
-                        uint32_t v[4];
+                    const uint16_t *q = src + (uint64_t)(row0 + r0) * ld + k;
+                    for (uint32_t i = 0; i < count; i += 8, q += 8 * ld) {  // 16 loads in flight
+                        uint16_t v[8], w[8];
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) {
-                            const uint32_t r = r0 + i + j;
-                            const uint16_t *q = src + (uint64_t)(row0 + r) * ld + k;
-                            v[j] = r < live && k < p.K ? q[0] : 0u;
-                            if (r < live && k + 1 < p.K) v[j] |= (uint32_t)q[1] << 16;
+                        for (uint32_t j = 0; j < 8; j++) {
+                            const bool there = i + j < count && r0 + i + j < live;
+                            v[j] = there && k < p.K ? q[j * ld] : 0;
+                            w[j] = there && k + 1 < p.K ? q[j * ld + 1] : 0;
                         }
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) {
+                        for (uint32_t j = 0; j < 8; j++) {
                             const uint32_t r = r0 + i + j;
-                            *reinterpret_cast<uint32_t *>(
-                                dst + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4) = v[j];
+                            if (i + j < count)
+                                *reinterpret_cast<uint32_t *>(dst + r * 128 +
+                                                              (((lane >> 2) ^ (r & 7u)) << 4) +
+                                                              (lane & 3u) * 4) =
+                                    v[j] | (uint32_t)w[j] << 16;
                         }
                     }
                 };
@@ -1721,6 +1743,43 @@ cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const Umma
     return cudaLaunchKernelEx(&c, kernel, tx, tw, u);
 }
 
+// How many clusters of 2 .. 8 CTAs, one to an SM, the device holds at once: a GPC
+// has room for whole ones only (clusters of 8: 8 to 16 of 18).  Asked once for
+// each device and size.
+uint32_t clusters_at_once(uint32_t size) {
+    static std::atomic<uint32_t> known[64][9];
+    int dev = 0;
+    if (size < 2 || cudaGetDevice(&dev) != cudaSuccess) return 0xffffffffu;
+    std::atomic<uint32_t> *const k = dev < 64 ? &known[dev][size] : nullptr;
+    if (k && k->load(std::memory_order_relaxed)) return k->load(std::memory_order_relaxed);
+    const auto kernel = linear_umma_kernel<FORM_DENSE, true, false, false>;
+    int n = 0;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(size);
+    c.blockDim = dim3(umma_threads(FORM_DENSE));
+    c.dynamicSmemBytes = SMEM_MIN;
+    c.attrs = attr;
+    c.numAttrs = launch_attributes(attr, size);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &c) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = 1;
+    }
+    if (k) k->store((uint32_t)n, std::memory_order_relaxed);
+    return (uint32_t)n;
+}
+
+// CTAs to a tile: the K range is split over a cluster where tiles leave half of
+// the SMs idle, as far as all clusters run at once.
+uint32_t split_of(uint64_t tiles, uint32_t sms, uint32_t kbs) {
+    if (tiles * 2 > sms) return 1;
+    uint32_t s = std::min<uint32_t>({8u, (uint32_t)(sms / tiles), kbs});
+    while (s > 1 && clusters_at_once(s) < tiles) s--;
+    return s;
+}
+
 // Rows per tile of M rows by nt feature tiles on `units` SMs or pairs of them:
 // the height whose waves of tiles take the least time, waves x (rows + what a
 // tile's K step costs beside its rows).
@@ -1771,8 +1830,7 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     if (pair) {
         grid = 2 * (uint32_t)std::min<uint64_t>(tiles, units);
     } else {
-        // fewer tiles than half the SMs: the K range is split over a cluster
-        if (tiles * 2 <= sms) u.split = std::min<uint32_t>({8u, (uint32_t)(sms / tiles), kbs});
+        u.split = split_of(tiles, sms, kbs);
         grid = u.split > 1 ? (uint32_t)tiles * u.split : (uint32_t)std::min<uint64_t>(tiles, sms);
     }
     u.tmem_stride = round_to(u.bn, 32);

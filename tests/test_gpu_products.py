@@ -117,7 +117,9 @@ SHAPES = [(1, 1, 32), (1, 8, 64), (1, 128, 4096), (1, 1000, 1024), (2, 130, 96),
           (127, 128, 448), (128, 128, 128), (129, 384, 512), (200, 1000, 608), (255, 130, 96),
           (256, 256, 1024), (257, 300, 640), (300, 2048, 256), (513, 640, 800), (1000, 1153, 320),
           # enough whole tiles for pairs of CTAs: a second half past the last feature, odd heights
-          (300, 19000, 96), (513, 9728, 160), (1030, 4900, 320), (700, 9600, 1056)]
+          (300, 19000, 96), (513, 9728, 160), (1030, 4900, 320), (700, 9600, 1056),
+          # more tiles than CTAs of a few rows, with one and with several K parts; half tiles
+          (3, 40000, 64), (12, 38000, 96), (7, 5000, 1600), (40, 520, 1024), (90, 260, 800)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -197,7 +199,8 @@ def sorted_sizes(kind, m, e, seed):
 @pytest.mark.parametrize("m,e,n,k", [(1, 1, 32, 32), (1, 8, 256, 512), (8, 8, 1000, 1024),
                                      (8, 64, 64, 96), (40, 3, 384, 2048), (96, 16, 130, 160),
                                      (257, 5, 200, 64), (1000, 7, 257, 320), (1500, 40, 128, 256),
-                                     (1500, 3, 7710, 160), (2100, 7, 2400, 320)])
+                                     (1500, 3, 7710, 160), (2100, 7, 2400, 320), (30, 9, 5200, 128),
+                                     (60, 2, 300, 1024)])
 @pytest.mark.parametrize("kind", ["even", "one", "ragged"])
 @pytest.mark.parametrize("form,dt,out", [("int4", "bf16", "bf16"), ("int4", "f16", "f32"),
                                          ("dense", "bf16", "f32"), ("dense", "f16", "f16")])
