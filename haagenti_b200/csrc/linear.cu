@@ -1218,17 +1218,20 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
             const uint32_t f = threadIdx.x % 16 * 8, base = smem_u32(smem);
             while (j < j1) {
                 float z[8] = {};
+                // parts in flight: a round of remote loads takes about 1400 clocks; the
+                // other forms have 80 registers
+                constexpr uint32_t FLY = TMA_W ? 8 : 4;
 #pragma unroll
-                for (uint32_t r0 = 0; r0 < 8; r0 += 4) {  // four parts in flight
-                    float4 a[4], b[4];
+                for (uint32_t r0 = 0; r0 < 8; r0 += FLY) {
+                    float4 a[FLY], b[FLY];
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++)
+                    for (uint32_t i = 0; i < FLY; i++)
                         if (r0 + i < u.split) {
                             a[i] = ld_cluster(base + (j * 128 + f) * 4, r0 + i);
                             b[i] = ld_cluster(base + (j * 128 + f + 4) * 4, r0 + i);
                         }
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++)
+                    for (uint32_t i = 0; i < FLY; i++)
                         if (r0 + i < u.split) {
                             z[0] += a[i].x, z[1] += a[i].y, z[2] += a[i].z, z[3] += a[i].w;
                             z[4] += b[i].x, z[5] += b[i].y, z[6] += b[i].z, z[7] += b[i].w;
