@@ -1375,21 +1375,26 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
     int *abort = reinterpret_cast<int *>(full + ST_WARPS * ST_SLOTS);
     const Groups groups(reinterpret_cast<uint32_t *>(abort + 2), p.E);
     const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < ST_WARPS * ST_SLOTS; i++) mbar_init(smem_u32(&full[i]), 1);
-        *abort = 0;
+    // a warp's barriers are its own: without groups it can start to load at once
+    if (lane == 0) {
+        for (int i = 0; i < ST_SLOTS; i++) mbar_init(smem_u32(&full[warp * ST_SLOTS + i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        *abort = 0;
     }
+    __syncwarp();
     after_previous_kernel();
-    if (warp == 1) scan_groups(p, q.tile, groups);
-    __syncthreads();
+    if (p.offsets) {
+        if (warp == 1) scan_groups(p, q.tile, groups);
+        __syncthreads();
+    }
     // the cluster's CTAs are all running before any of them writes to another
     if (q.split > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
     const uint32_t nt = q.nt.d, kbs = (uint32_t)pk_kblocks(p.K);
     const uint32_t rank = blockIdx.x & (q.split - 1), t = blockIdx.x >> q.shift;
-    const bool work = t < groups.first[p.E] * nt;  // of the whole cluster alike
+    // of the whole cluster alike
+    const bool work = !p.offsets || t < groups.first[p.E] * nt;
     uint32_t e = 0, m0 = 0, hi = 0, n0 = 0;
     float acc[8][NT][4];
 #pragma unroll
@@ -1401,9 +1406,14 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
     bool ok = true;
     if (work) {
         const uint32_t rt = q.nt.of(t);
-        e = p.E > 1 ? expert_of(groups.first, p.E, rt) : 0;
-        hi = groups.off[e + 1];
-        m0 = groups.off[e] + (rt - groups.first[e]) * ROWS;
+        if (p.offsets) {
+            e = p.E > 1 ? expert_of(groups.first, p.E, rt) : 0;
+            hi = groups.off[e + 1];
+            m0 = groups.off[e] + (rt - groups.first[e]) * ROWS;
+        } else {
+            hi = p.M;
+            m0 = rt * ROWS;
+        }
         n0 = (t - rt * nt) * 128;
         const uint32_t kb0 = kbs * rank >> q.shift, kb1 = kbs * (rank + 1) >> q.shift;
         const uint8_t *src = reinterpret_cast<const uint8_t *>(p.w) +
