@@ -4,7 +4,7 @@
 //
 // linear is grouped_linear with one expert that owns every row.  Weights are
 // dense matrices of x's type or INT4 payloads laid out by
-// hct_b200_int4_weight_pack (see Int4Block).
+// hct_b200_int4_weight_pack (the layout is described below).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -281,7 +281,7 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 constexpr int BK = 64;  // 128 bytes of a row: one swizzle row
 constexpr int A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8, MAX_RAW = 16;
-constexpr int SECTION = 4;
+constexpr int SECTION = 4;  // 256 products: at most 16 truncated sums
 constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KB
 constexpr uint32_t SMEM_MIN = 120 * 1024;  // one CTA per SM: TMEM is never waited for
 constexpr uint32_t RASTER = 8;
@@ -289,8 +289,8 @@ constexpr uint32_t EPI_BYTES = 2 * 16 * 128 * 4;  // staging of the two epilogue
 
 struct UmmaParams {
     LinParams p;
-    uint32_t bn;      // rows per tile at most (a multiple of xbox)
-    uint32_t xbox;    // rows per TMA box of x (a multiple of 16)
+    uint32_t bn;      // rows per tile at most
+    uint32_t xbox;    // rows per TMA box of x (a multiple of 8)
     uint32_t stages, raw_stages;
     uint32_t tmem_cols, tmem_stride;
     uint32_t split;   // CTAs per cluster, each a part of K
@@ -1575,6 +1575,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
 
 int code_of(cudaError_t e) {
     if (e == cudaSuccess) return HCT_B200_OK;
+    cudaGetLastError();  // it is reported here: nobody else finds it later
     if (e == cudaErrorMemoryAllocation) return HCT_B200_ERR_OUT_OF_MEMORY;
     if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) return HCT_B200_ERR_NO_DEVICE;
     return HCT_B200_ERR_CUDA;

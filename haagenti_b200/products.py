@@ -85,6 +85,8 @@ class Int4Weight:
         device = torch.device(device)
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream belongs to {stream.device}, the weight to {device}")
         with torch.cuda.device(device):
             stream = stream if stream is not None else torch.cuda.current_stream()
             with torch.cuda.stream(stream):
@@ -102,6 +104,7 @@ class Int4Weight:
         self.rows, self.cols = rows, cols
         self.experts = len(parts) if many else None
         self.packed = packed
+        self.home = stream.cuda_stream  # the stream that the memory's allocator knows of
         self.device = device
 
     @property
@@ -220,9 +223,12 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
         a.layout.pack_into(a.buffer, 0, m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride,
                            bias_ptr, gate_ptr, ldg, res_ptr, ldr, out.data_ptr(), out.stride(0),
                            off_ptr, experts, bits, x_tag, form, bias_tag, tag, activation, 0)
-        rc = fn(a.args, _raw_stream(dev))
+        raw = _raw_stream(dev)
+        rc = fn(a.args, raw)
         if rc:
             _check(rc)
+        if form and raw != weight.home:  # freed weights stay until this stream is done
+            wt.record_stream(torch.cuda.current_stream())
         return out
     with torch.cuda.device(dev):
         current = torch.cuda.current_stream()

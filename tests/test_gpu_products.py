@@ -496,6 +496,57 @@ def test_streams(hb, dev, form):
         assert torch.equal(o, want)
 
 
+def test_weight_freed_while_another_stream_reads_it(hb, dev):
+    """A weight laid out on one stream, used on another and dropped at once: its memory is not
+    handed out again before the product has read it."""
+    n, k, m = 4096, 4096, 300
+    data = payload_of(0.1 * torch.randn(n, k, device=dev))
+    x = torch.randn(m, k, device=dev).to(torch.bfloat16)
+    a, b = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+    want = hb.linear(x, hb.Int4Weight(data, n, k))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        w = hb.Int4Weight(data, n, k, stream=a)
+        size = w.packed.numel()
+        with torch.cuda.stream(b):
+            for _ in range(20):
+                y = hb.linear(x, w)
+        del w
+        with torch.cuda.stream(a):
+            junk = torch.full((size,), 255, dtype=torch.uint8, device=dev)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        del junk
+
+
+def test_two_threads(hb, dev):
+    """Calls from two threads at once, each on its own stream."""
+    import threading
+
+    n, k = 640, 1024
+    d = make(dev, 30, 200, n, k, 1, "int4", "bf16", "bf16", False, False, False)
+    w = hb.Int4Weight(d["w"][0], n, k)
+    want = {m: hb.linear(d["x"][:m], w) for m in (5, 200)}
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(m):
+        s = torch.cuda.Stream(dev)
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                y = hb.linear(d["x"][:m], w)
+        s.synchronize()
+        if not torch.equal(y, want[m]):
+            bad.append(m)
+
+    ts = [threading.Thread(target=work, args=(m,)) for m in (5, 200)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
 def test_reader_hands_out_its_int4_weight(hb, dev, orc):
     """A plain INT4 file multiplied from its payload equals the product with its decoded tensor."""
     from oracle import hct as OH
