@@ -208,7 +208,7 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
         ldr, res_ptr = _matrix(residual, "residual", shape, ot, dev), residual.data_ptr()
         grads |= residual.requires_grad
     if out is not None:
-        _matrix(out, "out", shape, ot, dev)
+        ldo = _matrix(out, "out", shape, ot, dev)
         grads |= out.requires_grad
     if grads and torch.is_grad_enabled():
         raise Unsupported(L.UNSUPPORTED, "the products have no backward pass: detach the tensors "
@@ -217,11 +217,12 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
     fn = lib.hct_b200_linear if offsets is None else lib.hct_b200_grouped_linear
     here = torch.cuda.current_device() == dev
     if here and stream is None:
-        if out is None:
-            out = x.new_empty(shape) if ot is xt else x.new_empty(shape, dtype=ot)
+        if out is None:  # sizes one by one: a tuple takes torch 1 us longer to read
+            out = x.new_empty(m, n) if ot is xt else torch.empty(m, n, dtype=ot, device=x.device)
+            ldo = n
         a = _ARGS
         a.layout.pack_into(a.buffer, 0, m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride,
-                           bias_ptr, gate_ptr, ldg, res_ptr, ldr, out.data_ptr(), out.stride(0),
+                           bias_ptr, gate_ptr, ldg, res_ptr, ldr, out.data_ptr(), ldo,
                            off_ptr, experts, bits, x_tag, form, bias_tag, tag, activation, 0)
         raw = _raw_stream(dev)
         rc = fn(a.args, raw)
