@@ -301,7 +301,7 @@ struct UmmaParams {
 struct Ctl {
     uint64_t xfull[MAX_STAGES], afull[MAX_STAGES], empty[MAX_STAGES];
     uint64_t rfull[MAX_RAW], rempty[MAX_RAW];
-    uint64_t tfull[2], tempty[2], drain;
+    uint64_t tfull[2], tempty[2], drain, parts;
     uint32_t tmem_base;
     int abort, issued, raw_issued;
 };
@@ -535,15 +535,13 @@ __device__ __forceinline__ void cluster_leave() {
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     asm volatile("barrier.cluster.wait;" ::: "memory");
 }
-__device__ __forceinline__ float4 ld_cluster(uint32_t saddr, uint32_t rank) {
-    uint32_t a;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(a)
-                 : "memory");
-    return v;
+// One bulk copy from this CTA's shared memory to another's, and to its barrier.
+__device__ __forceinline__ void push(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            to),
+        "r"(from), "r"(bytes), "r"(bar)
+        : "memory");
 }
 
 // One tile: expert, its rows [m0, m0 + rows) and first feature n0.
@@ -840,6 +838,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         }
         if (lane == 0) {
             mbar_init(smem_u32(&ctl->drain), u.issuers);
+            mbar_init(smem_u32(&ctl->parts), 1);
             ctl->abort = 0;
             ctl->issued = 0;
             ctl->raw_issued = 0;
@@ -1194,48 +1193,56 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
     }
 
     if (!PAIR && u.split > 1) {
-        // one tile per cluster: each CTA finishes its share of the tile's rows,
-        // adding the CTAs' parts in rank order.  Both barriers are reached by
-        // every thread of every CTA on every path.
+        // one tile per cluster: each CTA finishes its share of the tile's rows, adding the
+        // CTAs' parts in rank order.  A CTA pushes every other one its rows by one bulk
+        // copy (reading them there with ld.shared::cluster moved 6 to 8 bytes a clock: 10
+        // us for 196 rows).  The barriers and the wait are reached on every path
         constexpr int OUT = PRECISE ? OUT_F32 : OUT_16;
         Tile c{};
-        uint32_t j = 0, j1 = 0, n = 0;
+        uint32_t j = 0, j0 = 0, j1 = 0, n = 0;
         float bias[8];
         Operands o;
+        const uint32_t slot = (u.bn + u.split - 1) / u.split * 512;  // bytes that a CTA receives of one other
+        uint8_t *recv = smem + u.bn * 512;
         if (t0 < tiles) {
             c = tile_at<FEATURES>(u, groups, t0);
             n = c.n0 + threadIdx.x % 16 * 8;
-            j1 = n < p.N ? c.rows * (rank + 1) / u.split : 0;
-            j = c.rows * rank / u.split + threadIdx.x / 16;
-            if (j < j1) {
+            j0 = c.rows * rank / u.split;
+            j1 = c.rows * (rank + 1) / u.split;
+            j = j0 + threadIdx.x / 16;
+            if (j < j1 && n < p.N) {
                 load_bias8<BF>(p, c.e, n, bias);
                 load_operands<OUT>(p, c.m0 + j, n, o);
             }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the parts, for the copies
         __syncwarp();
-        cluster_barrier();
-        if (!aborted()) {
-            const uint32_t f = threadIdx.x % 16 * 8, base = smem_u32(smem);
+        cluster_barrier();  // every CTA's ring is free to receive
+        if (warp == 0 && lane < u.split && t0 < tiles) {
+            // lane r: the rows of CTA r
+            const uint32_t r0 = c.rows * lane / u.split, rows = c.rows * (lane + 1) / u.split - r0;
+            if (lane == rank) {
+                if (rows) mbar_expect_tx(smem_u32(&ctl->parts), rows * 512 * (u.split - 1));
+            } else if (rows) {
+                push(map_to(smem_u32(recv + (rank - (rank > lane)) * slot), lane), smem_u32(smem + r0 * 512), rows * 512,
+                     map_to(smem_u32(&ctl->parts), lane));
+            }
+        }
+        if (j1 > j0) {
+            const int go_on = 0;
+            if (!mbar_wait(smem_u32(&ctl->parts), 0, &go_on)) give_up();
+        }
+        if (!aborted() && n < p.N) {
+            const uint32_t f = threadIdx.x % 16 * 8;
             while (j < j1) {
                 float z[8] = {};
-                // parts in flight: a round of remote loads takes about 1400 clocks; the
-                // other forms have 80 registers
-                constexpr uint32_t FLY = TMA_W ? 8 : 4;
-#pragma unroll
-                for (uint32_t r0 = 0; r0 < 8; r0 += FLY) {
-                    float4 a[FLY], b[FLY];
-#pragma unroll
-                    for (uint32_t i = 0; i < FLY; i++)
-                        if (r0 + i < u.split) {
-                            a[i] = ld_cluster(base + (j * 128 + f) * 4, r0 + i);
-                            b[i] = ld_cluster(base + (j * 128 + f + 4) * 4, r0 + i);
-                        }
-#pragma unroll
-                    for (uint32_t i = 0; i < FLY; i++)
-                        if (r0 + i < u.split) {
-                            z[0] += a[i].x, z[1] += a[i].y, z[2] += a[i].z, z[3] += a[i].w;
-                            z[4] += b[i].x, z[5] += b[i].y, z[6] += b[i].z, z[7] += b[i].w;
-                        }
+                for (uint32_t r = 0; r < u.split; r++) {
+                    const uint8_t *from =
+                        r == rank ? smem + j * 512 : recv + (r - (r > rank)) * slot + (j - j0) * 512;
+                    const float4 a = reinterpret_cast<const float4 *>(from + f * 4)[0];
+                    const float4 b = reinterpret_cast<const float4 *>(from + f * 4)[1];
+                    z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w;
+                    z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) z[i] += bias[i];
@@ -1828,25 +1835,22 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     const uint64_t pair_tiles = (uint64_t)((p.N + 255) / 256) * ((p.M + 255) / 256 + (active - 1) / 2);
     const bool pair = !precise && !any && per_expert > 64 && pair_tiles * 2 >= sms;
     const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128, units = pair ? sms / 2 : sms;
-    uint64_t row_tiles;  // at most
-    if (grouped) {
-        u.bn = std::min(cap, pair || per_expert > 64 ? 256u : 128u);
-        u.xbox = 32;
-        row_tiles = p.M / u.bn + active;
-    } else {
-        u.bn = tile_rows(p.M, nt, units, cap);
-        u.xbox = pair ? u.bn / 2 : u.bn;
-        row_tiles = (p.M + u.bn - 1) / u.bn;
-    }
-    const uint64_t tiles = row_tiles * nt;
+    uint64_t tiles;  // at most
+    const auto plan = [&](uint32_t most) {
+        if (grouped) {
+            u.bn = std::min(most, pair || per_expert > 64 ? 256u : 128u);
+            u.xbox = 32;
+            tiles = (uint64_t)(p.M / u.bn + active) * nt;
+        } else {
+            u.bn = tile_rows(p.M, nt, units, most);
+            u.xbox = pair ? u.bn / 2 : u.bn;
+            tiles = (uint64_t)((p.M + u.bn - 1) / u.bn) * nt;
+        }
+    };
+    plan(cap);
+    // a split tile's parts, its own and the received ones, take the place of the ring
+    if (!pair && tiles * 2 <= sms && u.bn > 160) plan(160);
     if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
-    uint32_t grid;
-    if (pair) {
-        grid = 2 * (uint32_t)std::min<uint64_t>(tiles, units);
-    } else {
-        u.split = split_of(tiles, sms, kbs);
-        grid = u.split > 1 ? (uint32_t)tiles * u.split : (uint32_t)std::min<uint64_t>(tiles, sms);
-    }
     u.tmem_stride = round_to(u.bn, 32);
     // two issuers where their accumulators fit TMEM twice and an operand ring of 6
     // slots (any even number without groups) fits shared memory
@@ -1866,6 +1870,12 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     u.tile = Divisor(u.bn);
     u.nt = Divisor(nt);
     u.band = Divisor(nt * RASTER);
+    if (!pair) u.split = split_of(tiles, sms, kbs);
+    while (u.split > 1 && (u.bn + (u.bn + u.split - 1) / u.split * (u.split - 1)) * 512 > u.stages * stage)
+        u.split--;
+    const uint32_t grid = pair           ? 2 * (uint32_t)std::min<uint64_t>(tiles, units)
+                          : u.split > 1 ? (uint32_t)tiles * u.split
+                                        : (uint32_t)std::min<uint64_t>(tiles, sms);
     const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
 
     alignas(64) CUtensorMap tx{}, tw{};
