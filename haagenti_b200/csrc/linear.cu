@@ -1802,8 +1802,8 @@ uint32_t split_of(uint64_t tiles, uint32_t sms, uint32_t kbs) {
 }
 
 // Rows per tile of M rows by nt feature tiles on `units` SMs or pairs of them:
-// the height whose waves of tiles take the least time, waves x (rows + what a
-// tile's K step costs beside its rows).
+// the height whose waves of tiles take the least time, a K step being 2 clocks a
+// row and at least its issuing; the highest of those that are equal.
 uint32_t tile_rows(uint32_t M, uint32_t nt, uint32_t units, uint32_t cap) {
     if (M <= cap) return round_to(M, 16);
     uint32_t rows = cap;
@@ -1811,7 +1811,7 @@ uint32_t tile_rows(uint32_t M, uint32_t nt, uint32_t units, uint32_t cap) {
     for (uint32_t bn = cap; bn >= cap / 2; bn -= 16) {
         const uint64_t mts = (M + bn - 1) / bn;
         const uint32_t per = round_to((uint32_t)((M + mts - 1) / mts), 16);
-        const uint64_t cost = (mts * nt + units - 1) / units * (per + 32);
+        const uint64_t cost = (mts * nt + units - 1) / units * std::max(2 * per + 64, 550u);
         if (cost < best) {
             best = cost;
             rows = bn;
@@ -1835,7 +1835,9 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     const uint64_t pair_tiles = (uint64_t)((p.N + 255) / 256) * ((p.M + 255) / 256 + (active - 1) / 2);
     const bool pair = !precise && !any && per_expert > 64 && pair_tiles * 2 >= sms;
     const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128, units = pair ? sms / 2 : sms;
-    uint64_t tiles;  // at most
+    // everything of a plan that follows from the most rows that its tiles may have
+    uint64_t tiles = 0;  // at most
+    uint32_t fixed = 0, stage = 0;
     const auto plan = [&](uint32_t most) {
         if (grouped) {
             u.bn = std::min(most, pair || per_expert > 64 ? 256u : 128u);
@@ -1846,34 +1848,61 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
             u.xbox = pair ? u.bn / 2 : u.bn;
             tiles = (uint64_t)((p.M + u.bn - 1) / u.bn) * nt;
         }
+        // two issuers where their accumulators fit TMEM twice and an operand ring of 6
+        // slots (any even number without groups) fits shared memory
+        stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn / (pair ? 2 : 1) * 128;
+        u.issuers = u.bn <= (int4 ? 96u : 128u) && !(int4 && precise) ? 2 : 1;
+        u.raw_stages = !int4 ? 0 : u.issuers == 2 && u.bn > 64 ? 6 : 9;
+        const uint32_t other = u.raw_stages * PK_BYTES + EPI_BYTES;
+        fixed = 1024 + other + (uint32_t)sizeof(Ctl) + groups_bytes(p.E);
+        u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
+        if (u.issuers == 2) {
+            if (form == FORM_DENSE) u.stages &= ~1u;
+            else if (u.stages >= 6) u.stages = 6;
+            else u.issuers = 1;  // many experts' tables
+        }
+        // a split tile's parts, the CTA's own and those it receives, take the place of
+        // the rings and the staging, which are done with by then
+        u.split = pair ? 1 : split_of(tiles, sms, kbs);
+        while (u.split > 1 &&
+               (u.bn + (u.bn + u.split - 1) / u.split * (u.split - 1)) * 512 > u.stages * stage + other)
+            u.split--;
+    };
+    // Clocks of a plan, roughly: a K step takes its MMAs (2 a row), its issuing (300 with
+    // two issuers, else 550; INT4 550) or its bytes from L2 (50 a clock to an SM), and a
+    // split 2500 more and 40 for a row of its tile that is sent.
+    const auto clocks = [&] {
+        const uint32_t bytes = (int4 ? PK_BYTES : (uint32_t)A_BYTES) + u.bn * 128;
+        const uint64_t step = std::max({2 * u.bn, u.issuers == 2 && !int4 ? 300u : 550u, bytes / 50});
+        return (tiles * u.split + sms - 1) / sms * ((kbs + u.split - 1) / u.split) * step +
+               (u.split > 1 ? 2500 + 40 * u.bn * (u.split - 1) / u.split : 0);
     };
     plan(cap);
-    // a split tile's parts, its own and the received ones, take the place of the ring
-    if (!pair && tiles * 2 <= sms && u.bn > 160) plan(160);
+    if (!pair && tiles * 2 <= sms) {
+        // few tiles: lower ones may use more SMs (196 x 1792 x 1664: 112 rows and 5 parts
+        // of K 9.9 us, 208 rows and 4 parts 11.6) or not (256 x 8192 x 8192 INT4: 256
+        // rows and 2 parts 40 us, 128 rows 65)
+        const uint32_t rows = u.bn;
+        uint32_t best = cap;
+        uint64_t least = clocks();
+        for (const uint32_t most : {160u, 128u, 96u, 64u}) {
+            if (most >= rows) continue;
+            plan(most);
+            if (clocks() < least) {
+                least = clocks();
+                best = most;
+            }
+        }
+        plan(best);
+    }
     if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
     u.tmem_stride = round_to(u.bn, 32);
-    // two issuers where their accumulators fit TMEM twice and an operand ring of 6
-    // slots (any even number without groups) fits shared memory
-    const uint32_t stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn / (pair ? 2 : 1) * 128;
-    u.issuers = u.bn <= (int4 ? 96u : 128u) && !(int4 && precise) ? 2 : 1;
-    u.raw_stages = !int4 ? 0 : u.issuers == 2 && u.bn > 64 ? 6 : 9;
-    const uint32_t fixed = 1024 + u.raw_stages * PK_BYTES + EPI_BYTES + (uint32_t)sizeof(Ctl) +
-                           groups_bytes(p.E);
-    u.stages = std::min<uint32_t>(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
-    if (u.issuers == 2) {
-        if (form == FORM_DENSE) u.stages &= ~1u;
-        else if (u.stages >= 6) u.stages = 6;
-        else u.issuers = 1;  // many experts' tables
-    }
     u.tmem_cols = 64;
     while (u.tmem_cols < 2 * u.issuers * u.tmem_stride) u.tmem_cols *= 2;
     u.tile = Divisor(u.bn);
     u.nt = Divisor(nt);
     u.band = Divisor(nt * RASTER);
-    if (!pair) u.split = split_of(tiles, sms, kbs);
-    while (u.split > 1 && (u.bn + (u.bn + u.split - 1) / u.split * (u.split - 1)) * 512 > u.stages * stage)
-        u.split--;
-    const uint32_t grid = pair           ? 2 * (uint32_t)std::min<uint64_t>(tiles, units)
+    const uint32_t grid = pair          ? 2 * (uint32_t)std::min<uint64_t>(tiles, units)
                           : u.split > 1 ? (uint32_t)tiles * u.split
                                         : (uint32_t)std::min<uint64_t>(tiles, sms);
     const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
@@ -1980,8 +2009,13 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     const bool bf = a->x_dtype == HCT_B200_BF16, int4 = a->weight_form == HCT_B200_WEIGHT_INT4;
     const bool x_rows = tma_rows(p.x, p.M, p.ldx, p.K);
     if (int4) {
-        // the stream kernel for a few rows, and for any number of rows that TMA cannot fetch
-        if (!x_rows || p.M <= STREAM_ROWS * std::min(p.E, p.M)) return code_of(run_stream(p, bf, s));
+        // the stream kernel for a few rows, and for any number of rows that TMA cannot
+        // fetch; but not for many tiles of fewer K blocks than its warps (500 rows on 59
+        // experts of 23104 x 224: 160 us here, 248 there)
+        const uint32_t active = std::min(p.E, p.M);
+        const bool shorts = p.E > 1 && pk_kblocks(p.K) < ST_WARPS &&
+                            (uint64_t)active * ((p.N + 127) / 128) > 2ull * sm_count();
+        if (!x_rows || (p.M <= STREAM_ROWS * active && !shorts)) return code_of(run_stream(p, bf, s));
         return code_of(run_umma(p, grouped, FORM_INT4, bf, s));
     }
     const bool w_rows = tma_rows(p.w, p.N, p.ldw, p.K) &&
