@@ -1801,17 +1801,16 @@ uint32_t split_of(uint64_t tiles, uint32_t sms, uint32_t kbs) {
     return s;
 }
 
-// Rows per tile of M rows by nt feature tiles on `units` SMs or pairs of them:
-// the height whose waves of tiles take the least time, a K step being 2 clocks a
-// row and at least its issuing; the highest of those that are equal.
-uint32_t tile_rows(uint32_t M, uint32_t nt, uint32_t units, uint32_t cap) {
+// Rows per tile of M rows on pairs: the height whose waves of tiles take the least
+// time, a K step being 2 clocks a row and at least its issuing.
+uint32_t pair_rows(uint32_t M, uint32_t nt, uint32_t pairs, uint32_t cap) {
     if (M <= cap) return round_to(M, 16);
     uint32_t rows = cap;
     uint64_t best = ~0ull;
     for (uint32_t bn = cap; bn >= cap / 2; bn -= 16) {
         const uint64_t mts = (M + bn - 1) / bn;
         const uint32_t per = round_to((uint32_t)((M + mts - 1) / mts), 16);
-        const uint64_t cost = (mts * nt + units - 1) / units * std::max(2 * per + 64, 550u);
+        const uint64_t cost = (mts * nt + pairs - 1) / pairs * std::max(2 * per + 64, 550u);
         if (cost < best) {
             best = cost;
             rows = bn;
@@ -1834,20 +1833,14 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     // pairs where tiles of 256 features keep every pair busy
     const uint64_t pair_tiles = (uint64_t)((p.N + 255) / 256) * ((p.M + 255) / 256 + (active - 1) / 2);
     const bool pair = !precise && !any && per_expert > 64 && pair_tiles * 2 >= sms;
-    const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128, units = pair ? sms / 2 : sms;
-    // everything of a plan that follows from the most rows that its tiles may have
+    const uint32_t nt = pair ? (p.N + 255) / 256 : (p.N + 127) / 128;
+    // everything of a plan that follows from the rows that its tiles may have
     uint64_t tiles = 0;  // at most
     uint32_t fixed = 0, stage = 0;
-    const auto plan = [&](uint32_t most) {
-        if (grouped) {
-            u.bn = std::min(most, pair || per_expert > 64 ? 256u : 128u);
-            u.xbox = 32;
-            tiles = (uint64_t)(p.M / u.bn + active) * nt;
-        } else {
-            u.bn = tile_rows(p.M, nt, units, most);
-            u.xbox = pair ? u.bn / 2 : u.bn;
-            tiles = (uint64_t)((p.M + u.bn - 1) / u.bn) * nt;
-        }
+    const auto plan = [&](uint32_t rows) {
+        u.bn = rows;
+        u.xbox = grouped ? 32 : pair ? rows / 2 : rows;
+        tiles = (grouped ? (uint64_t)(p.M / rows + active) : (uint64_t)((p.M + rows - 1) / rows)) * nt;
         // two issuers where their accumulators fit TMEM twice and an operand ring of 6
         // slots (any even number without groups) fits shared memory
         stage = (int4 && precise ? 2 : 1) * A_BYTES + u.bn / (pair ? 2 : 1) * 128;
@@ -1877,20 +1870,34 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
         return (tiles * u.split + sms - 1) / sms * ((kbs + u.split - 1) / u.split) * step +
                (u.split > 1 ? 2500 + 40 * u.bn * (u.split - 1) / u.split : 0);
     };
-    plan(cap);
-    if (!pair && tiles * 2 <= sms) {
-        // few tiles: lower ones may use more SMs (196 x 1792 x 1664: 112 rows and 5 parts
-        // of K 9.9 us, 208 rows and 4 parts 11.6) or not (256 x 8192 x 8192 INT4: 256
-        // rows and 2 parts 40 us, 128 rows 65)
-        const uint32_t rows = u.bn;
-        uint32_t best = cap;
-        uint64_t least = clocks();
-        for (const uint32_t most : {160u, 128u, 96u, 64u}) {
-            if (most >= rows) continue;
-            plan(most);
+    if (pair) {
+        plan(grouped ? cap : pair_rows(p.M, nt, sms / 2, cap));
+    } else {
+        // Lower tiles may use more SMs (196 x 1792 x 1664: 112 rows and 5 parts of K 9.9
+        // us, 208 rows and 4 parts 11.6) or not (256 x 8192 x 8192 INT4: 256 rows and 2
+        // parts 40 us, 128 rows 65).  linear: M in 1 to 6 tiles more than it needs;
+        // grouped, whose groups are not known here: some heights
+        uint32_t best = 0;
+        uint64_t least = ~0ull;
+        const auto consider = [&](uint32_t rows) {
+            plan(rows);
             if (clocks() < least) {
                 least = clocks();
-                best = most;
+                best = rows;
+            }
+        };
+        if (grouped) {
+            const uint32_t most = std::min(cap, per_expert > 64 ? 256u : 128u);
+            for (uint32_t rows = most; rows >= 64; rows -= 32) {
+                consider(rows);
+                if (tiles * 2 > sms) break;
+            }
+        } else {
+            const uint32_t needed = (p.M + cap - 1) / cap;
+            for (uint32_t mts = needed; mts < needed + 7; mts++) {
+                const uint32_t rows = round_to((p.M + mts - 1) / mts, 16);
+                if (rows < 48 && mts > needed) break;
+                consider(rows);
             }
         }
         plan(best);
@@ -1902,7 +1909,7 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     u.tile = Divisor(u.bn);
     u.nt = Divisor(nt);
     u.band = Divisor(nt * RASTER);
-    const uint32_t grid = pair          ? 2 * (uint32_t)std::min<uint64_t>(tiles, units)
+    const uint32_t grid = pair          ? 2 * (uint32_t)std::min<uint64_t>(tiles, sms / 2)
                           : u.split > 1 ? (uint32_t)tiles * u.split
                                         : (uint32_t)std::min<uint64_t>(tiles, sms);
     const uint32_t smem = std::max(SMEM_MIN, fixed + u.stages * stage);
