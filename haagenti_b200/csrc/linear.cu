@@ -795,9 +795,14 @@ __device__ __forceinline__ void load_bias8(const LinParams &p, uint32_t e, uint3
     for (int j = 0; j < 8; j++) bias[j] = n + j < p.N ? bias_of<BF>(p, e, n + j) : 0.0f;
 }
 
+__device__ __forceinline__ void prefetch_l2(const void *q) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+}
+
 // Where the operands come from: dense matrices by TMA, packed INT4 weights (x by
-// TMA), or dense matrices of any stride and alignment, copied by warps.
-enum { FORM_DENSE = 0, FORM_INT4 = 1, FORM_ANY = 2 };
+// TMA), or dense matrices of any stride and alignment, copied by warps, whose loads
+// are 4 bytes wide where every row starts on 4 bytes and K is even, else 2.
+enum { FORM_DENSE = 0, FORM_INT4 = 1, FORM_ANY = 2, FORM_WORDS = 3 };
 constexpr int umma_threads(int form) { return form == FORM_DENSE ? 384 : 768; }
 // rows per tile at most: a thread of the epilogue keeps half of them as f32 sums where PRECISE
 __host__ __device__ constexpr uint32_t max_rows(int form, bool precise) {
@@ -808,7 +813,8 @@ template <int FORM, bool BF, bool PRECISE, bool PAIR>
 __global__ void __launch_bounds__(umma_threads(FORM), 1)
     linear_umma_kernel(const __grid_constant__ CUtensorMap tmX,
                        const __grid_constant__ CUtensorMap tmW, const __grid_constant__ UmmaParams u) {
-    constexpr bool INT4 = FORM == FORM_INT4, ANY = FORM == FORM_ANY, TMA_W = FORM == FORM_DENSE;
+    constexpr bool INT4 = FORM == FORM_INT4, WORDS = FORM == FORM_WORDS, ANY = WORDS || FORM == FORM_ANY,
+                   TMA_W = FORM == FORM_DENSE;
     constexpr uint32_t A_PARTS = INT4 && PRECISE ? 2 : 1;
     constexpr uint32_t GROUPS = 3;  // of dequantising or loading warps
     constexpr uint32_t FEATURES = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
@@ -1070,25 +1076,38 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                 const auto copy = [&](const uint16_t *src, uint64_t ld, uint32_t row0, uint32_t live,
                                       uint32_t r0, uint32_t count, uint8_t *dst) {
                     const uint16_t *q = src + (uint64_t)(row0 + r0) * ld + k;
-                    for (uint32_t i = 0; i < count; i += 8, q += 8 * ld) {  // 16 loads in flight
-                        uint16_t v[8], w[8];
+                    constexpr uint32_t N = WORDS ? 16 : 8;  // 16 loads in flight
+                    for (uint32_t i = 0; i < count; i += N, q += N * ld) {
+                        uint32_t v[N];
+                        uint16_t hi[N];
 #pragma unroll
-                        for (uint32_t j = 0; j < 8; j++) {
+                        for (uint32_t j = 0; j < N; j++) {
                             const bool there = i + j < count && r0 + i + j < live;
-                            v[j] = there && k < p.K ? q[j * ld] : 0;
-                            w[j] = there && k + 1 < p.K ? q[j * ld + 1] : 0;
+                            if (WORDS) {
+                                v[j] = there && k < p.K ? *reinterpret_cast<const uint32_t *>(q + j * ld) : 0;
+                            } else {
+                                v[j] = there && k < p.K ? q[j * ld] : 0;
+                                hi[j] = there && k + 1 < p.K ? q[j * ld + 1] : 0;
+                            }
                         }
 #pragma unroll
-                        for (uint32_t j = 0; j < 8; j++) {
+                        for (uint32_t j = 0; j < N; j++) {
                             const uint32_t r = r0 + i + j;
                             if (i + j < count)
                                 *reinterpret_cast<uint32_t *>(dst + r * 128 +
                                                               (((lane >> 2) ^ (r & 7u)) << 4) +
                                                               (lane & 3u) * 4) =
-                                    v[j] | (uint32_t)w[j] << 16;
+                                    WORDS ? v[j] : v[j] | (uint32_t)hi[j] << 16;
                         }
                     }
                 };
+                // the group's next K step on its way to L2 meanwhile
+                if (kb + GROUPS < kb1) {
+                    const uint32_t next = (kb + GROUPS) * BK, row = c.n0 + part * 32 + lane;
+                    if (row < p.N) prefetch_l2(w + (uint64_t)row * p.ldw + next);
+                    for (uint32_t r = part * quarter + lane; r < min((part + 1) * quarter, c.rows); r += 32)
+                        prefetch_l2(x + (uint64_t)(c.m0 + r) * p.ldx + next);
+                }
                 copy(w, p.ldw, c.n0, p.N - c.n0, part * 32, 32, a);
                 copy(x, p.ldx, c.m0, c.rows, part * quarter, quarter, a + A_BYTES);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1822,7 +1841,7 @@ uint32_t pair_rows(uint32_t M, uint32_t nt, uint32_t pairs, uint32_t cap) {
 // Pair or single, tile height, split and ring depths of a call on the
 // tensor-core kernel.
 cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaStream_t s) {
-    const bool int4 = form == FORM_INT4, any = form == FORM_ANY;
+    const bool int4 = form == FORM_INT4, any = form >= FORM_ANY;
     const bool precise = p.odt == HCT_B200_F32;
     const uint32_t sms = (uint32_t)sm_count(), cap = max_rows(form, precise);
     const uint32_t kbs = std::max((p.K + BK - 1) / BK, 1u);
@@ -1926,7 +1945,7 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
         constexpr int F = decltype(form_)::value;
         constexpr bool B = decltype(bf_)::value;
         if (precise) return launch_umma<F, B, true, false>(tx, tw, u, grid, smem, s);
-        if constexpr (F != FORM_ANY)
+        if constexpr (F < FORM_ANY)
             if (pair) return launch_umma<F, B, false, true>(tx, tw, u, grid, smem, s);
         return launch_umma<F, B, false, false>(tx, tw, u, grid, smem, s);
     };
@@ -1934,7 +1953,8 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
         return bf ? launch(form_, std::true_type()) : launch(form_, std::false_type());
     };
     if (int4) return typed(std::integral_constant<int, FORM_INT4>());
-    if (any) return typed(std::integral_constant<int, FORM_ANY>());
+    if (form == FORM_ANY) return typed(std::integral_constant<int, FORM_ANY>());
+    if (form == FORM_WORDS) return typed(std::integral_constant<int, FORM_WORDS>());
     return typed(std::integral_constant<int, FORM_DENSE>());
 }
 
@@ -2027,7 +2047,12 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     }
     const bool w_rows = tma_rows(p.w, p.N, p.ldw, p.K) &&
                         (p.E == 1 || (p.w_stride % 8 == 0 && p.w_stride && p.w_stride < 1ull << 38));
-    return code_of(run_umma(p, grouped, p.K && x_rows && w_rows ? FORM_DENSE : FORM_ANY, bf, s));
+    if (p.K && x_rows && w_rows) return code_of(run_umma(p, grouped, FORM_DENSE, bf, s));
+    // rows that TMA cannot fetch (500 x 5000 x 4002: 129 us with loads of 4 bytes, 203 of 2)
+    const bool words = ((uintptr_t)p.x | (uintptr_t)p.w) % 4 == 0 && p.K % 2 == 0 &&
+                       (p.M == 1 || p.ldx % 2 == 0) && (p.N == 1 || p.ldw % 2 == 0) &&
+                       (p.E == 1 || p.w_stride % 2 == 0);
+    return code_of(run_umma(p, grouped, words ? FORM_WORDS : FORM_ANY, bf, s));
 }
 
 }  // namespace

@@ -695,3 +695,24 @@ def test_python_refusals(hb, dev):
 
 def test_status_is_clean(hb):
     hb.linear_status()
+
+
+@pytest.mark.parametrize("shift", [1, 2])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 2), (5, 130, 66), (80, 64, 1502), (150, 300, 994), (20, 5000, 1000)])
+@pytest.mark.parametrize("dt,out", [("bf16", "bf16"), ("f16", "f32")])
+def test_dense_rows_at_any_place(hb, dev, shift, m, n, k, dt, out):
+    """Rows that start on 2 or on 4 bytes, even and odd strides between them, NaN around them."""
+    for pad in (6, 7):
+        d = make(dev, m + n + k, m, n, k, 2, "dense", dt, out, False, False, False)
+        x = torch.full((m, k + pad), float("nan"), device=dev, dtype=DT[dt])[:, shift:shift + k]
+        w = torch.full((2, n + 1, k + pad), float("nan"), device=dev, dtype=DT[dt])[:, :n, shift:shift + k]
+        x.copy_(d["x"])
+        w.copy_(torch.stack(d["w"]))
+        want, tol = define(x, w[0], None, 0, None, None, DT[out], False)
+        check(hb.linear(x, w[0], out_dtype=TAG[out]), want, tol)
+        cut = m // 3
+        off = torch.tensor([0, cut, m], dtype=torch.int32, device=dev)
+        want2, tol2 = define(x, w[1], None, 0, None, None, DT[out], False)
+        got = hb.grouped_linear(x, w, off, out_dtype=TAG[out])
+        check(got, torch.cat([want[:cut], want2[cut:]]), torch.cat([tol[:cut], tol2[cut:]]))
+    hb.linear_status()
