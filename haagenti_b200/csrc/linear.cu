@@ -250,7 +250,7 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 //   warps 12-23 INT4: three groups of 128 threads dequantise every third K step,
 //               a thread per weight row, into the 128B-swizzled A tile.  Dense
 //               rows that TMA cannot fetch (unaligned starts, odd strides): they
-//               copy both operands by plain loads
+//               copy both operands by loads of 4 or of 2 bytes
 //
 // PAIR: where whole tiles of rows keep every SM busy, two CTAs share one tile of
 // 256 features (cta_group::2): each holds the weights of its 128 features and
@@ -260,8 +260,10 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 // With at least one tile per SM the kernel is persistent (grid = SMs) and the
 // accumulators are double-buffered, so a tile's epilogue runs under the next
 // tile's MMAs.  With fewer, the K range of a tile is split over a cluster of
-// CTAs, whose partial sums meet in distributed shared memory and are added in
-// rank order: no workspace, no atomics, the same bits every time.
+// CTAs: each pushes the rows that another finishes into that one's shared memory
+// by bulk copies (reading them there took 6 to 8 bytes a clock: 196 x 1792 x 1664
+// 17.6 us, pushed 9.6), and a row's parts are added in rank order: no workspace,
+// no atomics, the same bits every time.
 //
 // F32 outputs (PRECISE) accumulate at most SECTION K steps in TMEM and add the
 // sections in registers with rounding; INT4 weights are then two A operands,
@@ -1881,11 +1883,13 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
             u.split--;
     };
     // Clocks of a plan, roughly: a K step takes its MMAs (2 a row), its issuing (300 with
-    // two issuers, else 550; INT4 550) or its bytes from L2 (50 a clock to an SM), and a
-    // split 2500 more and 40 for a row of its tile that is sent.
+    // two issuers, else 550; INT4 550), its bytes from L2 (50 a clock to an SM) or the copies
+    // of its rows by warps (17 each, 11 in words; 4096 x 4096 x 1001 217 us, K = 1004 143), and
+    // a split 2500 more and 40 for a row of its tile that is sent.
     const auto clocks = [&] {
         const uint32_t bytes = (int4 ? PK_BYTES : (uint32_t)A_BYTES) + u.bn * 128;
-        const uint64_t step = std::max({2 * u.bn, u.issuers == 2 && !int4 ? 300u : 550u, bytes / 50});
+        const uint64_t step = any ? (128 + u.bn) * (form == FORM_ANY ? 17 : 11)
+                                  : std::max({2 * u.bn, u.issuers == 2 && !int4 ? 300u : 550u, bytes / 50});
         return (tiles * u.split + sms - 1) / sms * ((kbs + u.split - 1) / u.split) * step +
                (u.split > 1 ? 2500 + 40 * u.bn * (u.split - 1) / u.split : 0);
     };
@@ -1894,7 +1898,8 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     } else {
         // Lower tiles may use more SMs (196 x 1792 x 1664: 112 rows and 5 parts of K 9.9
         // us, 208 rows and 4 parts 11.6) or not (256 x 8192 x 8192 INT4: 256 rows and 2
-        // parts 40 us, 128 rows 65).  linear: M in 1 to 6 tiles more than it needs;
+        // parts 40 us, 128 rows 65).  linear: M in up to 6 tiles more than it needs,
+        // of 48 rows or more (16 where copying bounds: 80 x 64 x 12511 39 us, 45 in one tile);
         // grouped, whose groups are not known here: some heights
         uint32_t best = 0;
         uint64_t least = ~0ull;
@@ -1915,7 +1920,7 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
             const uint32_t needed = (p.M + cap - 1) / cap;
             for (uint32_t mts = needed; mts < needed + 7; mts++) {
                 const uint32_t rows = round_to((p.M + mts - 1) / mts, 16);
-                if (rows < 48 && mts > needed) break;
+                if (rows < (any ? 16u : 48u) && mts > needed) break;
                 consider(rows);
             }
         }

@@ -261,7 +261,8 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * be infinite where x is F16.
  *
  * Strides are in elements.  Rows of x and w that start on 16-byte boundaries
- * take the tensor-core path; others are handled by a slower kernel.  out may
+ * are fetched by TMA; others are copied by plain loads, several times slower
+ * (4-byte loads where rows start on 4 bytes and in_features is even).  out may
  * be the same matrix as gate or residual (same pointer, stride and type); any
  * other overlap of out with an input is HCT_B200_ERR_INVALID_ARGUMENT, as are
  * out rows that overlap one another.  rows == 0 or out_features == 0 is a
