@@ -13,6 +13,10 @@ slope: gelu's is at most 1.13):
 
 Where the bounds add up, |gate| multiplies all but the last.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -716,3 +720,33 @@ def test_dense_rows_at_any_place(hb, dev, shift, m, n, k, dt, out):
         got = hb.grouped_linear(x, w, off, out_dtype=TAG[out])
         check(got, torch.cat([want[:cut], want2[cut:]]), torch.cat([tol[:cut], tol2[cut:]]))
     hb.linear_status()
+
+
+COLD = """
+import torch, haagenti_b200 as H
+dev = torch.device("cuda", 0)
+m, n, k, form, out = {case}
+x = torch.ones(m, k, device=dev, dtype=torch.bfloat16)
+if form == "int4":
+    s = torch.full((n * k // 32,), 0.5, dtype=torch.float16, device=dev).view(torch.uint8)
+    w = H.Int4Weight(torch.cat([s, torch.full((n * k // 2,), 0x99, dtype=torch.uint8, device=dev)]), n, k)
+else:
+    w = torch.full((n, k), 0.5, device=dev, dtype=torch.bfloat16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = H.linear(x, w, out_dtype=out)
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 0.5 * k).all()
+H.linear_status()
+"""
+
+
+@pytest.mark.parametrize("case", [(1, 256, 1024, "int4", None), (40, 256, 1024, "int4", 0),
+                                  (40, 256, 1024, "dense", None), (3, 256, 130, "dense", None),
+                                  (4096, 2560, 256, "dense", None)])
+def test_first_call_of_a_process_captured(hb, dev, case):
+    """A graph may hold the first product of a process: nothing has been set up before."""
+    subprocess.run([sys.executable, "-c", COLD.format(case=case)], check=True, timeout=300,
+                   cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
