@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -267,7 +268,10 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 //
 // F32 outputs (PRECISE) accumulate at most SECTION K steps in TMEM and add the
 // sections in registers with rounding; INT4 weights are then two A operands,
-// the rounded weight and what the rounding left.
+// the rounded weight and what the rounding left, each with accumulators of its
+// own.  Where a value of x is infinite, the rounded weights alone give the sum
+// that the weights would (a weight is 0 where its rounding is), and the sum of
+// what was left, with infinity times 0 or infinities of both signs, is dropped.
 //
 // A wait on a slot's parity is sound only for one that cannot be two passes
 // behind.  The producers and issuers meet every pass of a slot in order.  The
@@ -942,7 +946,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                 ok = mbar_wait_warp(smem_u32(&ctl->tempty[acc.slot]), acc.pass ^ 1u, &ctl->abort);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + (acc.slot * u.issuers + me) * u.tmem_stride;
+                const uint32_t d = tmem + (acc.slot * u.issuers * A_PARTS + me) * u.tmem_stride;
                 while (kb < end) {
                     if ((at.slot & every) != me) {
                         kb++, at.step();
@@ -963,8 +967,8 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                         for (uint32_t a = 0; a < A_PARTS; a++)
 #pragma unroll
                             for (uint32_t k = 0; k < BK / 16; k++)
-                                umma<PAIR>(d, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k, idesc,
-                                           more || a || k);
+                                umma<PAIR>(d + a * u.tmem_stride, da + a * (A_BYTES >> 4) + 2 * k, db + 2 * k,
+                                           idesc, more || k);
                         umma_commit<PAIR>(smem_u32(&ctl->empty[slot]));
                     };
                     if (elect_one()) {
@@ -1147,8 +1151,8 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                 // a section of one K step is in the accumulators of that step's issuer
                 const bool two = u.issuers == 2 && kb + 1 < kb1;
                 const uint32_t lone = two ? 0 : steps & (u.issuers - 1);
-                const uint32_t ta =
-                    tmem + (acc.slot * u.issuers + lone) * u.tmem_stride + ((q * 32) << 16);
+                const uint32_t ta = tmem + (acc.slot * u.issuers * A_PARTS + lone) * u.tmem_stride +
+                                    ((q * 32) << 16);
                 steps += min(sect, kb1 - kb);
                 if (PRECISE) {
 #pragma unroll
@@ -1160,10 +1164,13 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                         tmem_ld16(ta + j0, v);
 #pragma unroll
                         for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
-                        if (two) {
+                        if (two || A_PARTS == 2) {
                             tmem_ld16(ta + u.tmem_stride + j0, v);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
+                            for (int j = 0; j < 16; j++) {
+                                const float f = __uint_as_float(v[j]);
+                                sum[i][j] += A_PARTS == 1 || fabsf(f) < INFINITY ? f : 0.0f;
+                            }
                         }
                     }
                 } else {
@@ -1929,7 +1936,7 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     if (tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
     u.tmem_stride = round_to(u.bn, 32);
     u.tmem_cols = 64;
-    while (u.tmem_cols < 2 * u.issuers * u.tmem_stride) u.tmem_cols *= 2;
+    while (u.tmem_cols < 2 * u.issuers * (int4 && precise ? 2 : 1) * u.tmem_stride) u.tmem_cols *= 2;
     u.tile = Divisor(u.bn);
     u.nt = Divisor(nt);
     u.band = Divisor(nt * RASTER);

@@ -750,3 +750,25 @@ def test_first_call_of_a_process_captured(hb, dev, case):
     """A graph may hold the first product of a process: nothing has been set up before."""
     subprocess.run([sys.executable, "-c", COLD.format(case=case)], check=True, timeout=300,
                    cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+@pytest.mark.parametrize("form,dt,out", [("int4", "bf16", "f32"), ("int4", "f16", "f32"),
+                                         ("int4", "bf16", "bf16"), ("int4", "f16", "f16"),
+                                         ("dense", "bf16", "f32"), ("dense", "f16", "f16")])
+@pytest.mark.parametrize("m,k", [(4, 320), (16, 1024), (40, 320), (40, 4096), (300, 320)])
+def test_infinite_inputs_give_what_the_definition_gives(hb, dev, form, dt, out, m, k):
+    """Infinity times a weight has the weight's sign, times zero it is NaN, and infinities of both
+    signs are NaN, for however many rows; the other rows keep their values."""
+    n = 160
+    d = make(dev, m + k, m, n, k, 1, form, dt, out, False, False, False)
+    x, inf = d["x"], float("inf")
+    x[1, 17], x[2, 5] = inf, -inf
+    x[3, 40], x[3, 200] = inf, -inf
+    got = run_linear(hb, d, n, k, form, 0, out)
+    w = weight64(d["w"][0], n, k) if form == "int4" else d["w"][0]
+    want, tol = define(x, w, None, 0, None, None, DT[out], form == "int4")
+    bad = torch.tensor([1, 2, 3], device=dev)
+    a, b = got[bad].double(), want[bad]
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
+    keep = [i for i in range(m) if i not in (1, 2, 3)]
+    check(got[keep], want[keep], tol[keep])
