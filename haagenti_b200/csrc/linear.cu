@@ -580,19 +580,37 @@ __device__ __forceinline__ Tile tile_at(const UmmaParams &u, const Groups &g, ui
 // the scale, rounded once.  bf16: the f16 scale (11 bits) is hi + lo, two
 // bf16 values; (n - 8) lo has at most 6 bits, so fma(n - 8, hi, (n - 8) lo)
 // rounds the exact product once.
-template <bool BF>
+//
+// fp16 and PRECISE: a weight is 8 h + l with h = (n - 8) / 8 s rounded, which is in
+// range for every finite scale, and l = 8 ((n - 8) / 8 s - h), which has at most 5
+// bits and no bit below 2^-24: exact.  To keep every step of l in range too, it is
+// 8 fma((n - 8) / 8, s, -h) for scales of 2^-8 and more, and fma((n - 8) / 8, 8 s,
+// -8 h) for smaller ones.  h takes a scale of 2^-21 in the place of smaller ones, so
+// that it is 0 only where the weight is.
+template <bool BF, bool PRECISE>
 struct Scale;
 template <>
-struct Scale<false> {
+struct Scale<false, false> {
     __half2 s;
-    bool finite;
-    __device__ __forceinline__ explicit Scale(uint16_t b) {
-        s = __half2half2(__ushort_as_half(b));
-        finite = (b & 0x7c00u) != 0x7c00u;
-    }
+    __device__ __forceinline__ explicit Scale(uint16_t b) : s(__half2half2(__ushort_as_half(b))) {}
 };
 template <>
-struct Scale<true> {
+struct Scale<false, true> {
+    __half2 h, s, minus, times;  // l = times fma(n, s, minus h)
+    bool finite;
+    __device__ __forceinline__ explicit Scale(uint16_t b) {
+        const uint16_t mag = b & 0x7fffu, sign = b & 0x8000u;
+        finite = mag < 0x7c00u;
+        h = __half2half2(__ushort_as_half(mag != 0 && mag < 8 ? (uint16_t)(sign | 8) : b));
+        const bool large = mag >= 0x1c00u;  // 2^-8
+        s = __half2half2(__ushort_as_half(b));
+        if (!large) s = __hmul2(s, __float2half2_rn(8.0f));
+        minus = __float2half2_rn(large ? -1.0f : -8.0f);
+        times = __float2half2_rn(large ? 8.0f : 1.0f);
+    }
+};
+template <bool PRECISE>
+struct Scale<true, PRECISE> {
     __nv_bfloat162 hi, lo;
     bool finite;
     __device__ __forceinline__ explicit Scale(uint16_t b) {
@@ -603,24 +621,36 @@ struct Scale<true> {
         lo = __bfloat162bfloat162(__float2bfloat16_rn(finite ? f - __bfloat162float(h) : 0.0f));
     }
 };
-template <bool PRECISE>
-__device__ __forceinline__ void dequant8(uint32_t w, const Scale<false> &s, uint32_t (&v)[4],
+// odd pairs stay where they are: 1024 + 16 n, whose sixteenth less 72 is n - 8
+__device__ __forceinline__ __half2 fp16_pair(uint32_t w, int j) {
+    uint32_t b = (j & 1 ? (w >> (8 * (j / 2))) & 0x00f000f0u : (w >> (8 * (j / 2))) & 0x000f000fu) |
+                 0x64006400u;
+    return *reinterpret_cast<__half2 *>(&b);
+}
+__device__ __forceinline__ void dequant8(uint32_t w, const Scale<false, false> &s, uint32_t (&v)[4],
+                                         uint32_t (&)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const __half2 m = fp16_pair(w, j);
+        const __half2 n = j & 1 ? __hfma2(m, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
+                                : __hsub2(m, __float2half2_rn(1032.0f));
+        v[j] = bits_of(__hmul2(n, s.s));
+    }
+}
+__device__ __forceinline__ void dequant8(uint32_t w, const Scale<false, true> &s, uint32_t (&v)[4],
                                          uint32_t (&l)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        // odd pairs stay where they are: 1024 + 16 n, whose sixteenth less 72 is n - 8
-        uint32_t b = (j & 1 ? (w >> (8 * (j / 2))) & 0x00f000f0u : (w >> (8 * (j / 2))) & 0x000f000fu) |
-                     0x64006400u;
-        const __half2 m = *reinterpret_cast<__half2 *>(&b);
-        const __half2 n = j & 1 ? __hfma2(m, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f))
-                                : __hsub2(m, __float2half2_rn(1032.0f));
-        const __half2 h = __hmul2(n, s.s);
+        const __half2 m = fp16_pair(w, j);  // 1024 + n or 1024 + 16 n; here to (n - 8) / 8, exactly
+        const __half2 n = j & 1 ? __hfma2(m, __float2half2_rn(0.0078125f), __float2half2_rn(-9.0f))
+                                : __hfma2(m, __float2half2_rn(0.125f), __float2half2_rn(-129.0f));
+        const __half2 h = __hmul2(n, s.h);
         v[j] = bits_of(h);
-        if (PRECISE) l[j] = s.finite ? bits_of(__hfma2(n, s.s, __hneg2(h))) : 0u;
+        l[j] = s.finite ? bits_of(__hmul2(__hfma2(n, s.s, __hmul2(h, s.minus)), s.times)) : 0u;
     }
 }
 template <bool PRECISE>
-__device__ __forceinline__ void dequant8(uint32_t w, const Scale<true> &s, uint32_t (&v)[4],
+__device__ __forceinline__ void dequant8(uint32_t w, const Scale<true, PRECISE> &s, uint32_t (&v)[4],
                                          uint32_t (&l)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -822,6 +852,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
     constexpr bool INT4 = FORM == FORM_INT4, WORDS = FORM == FORM_WORDS, ANY = WORDS || FORM == FORM_ANY,
                    TMA_W = FORM == FORM_DENSE;
     constexpr uint32_t A_PARTS = INT4 && PRECISE ? 2 : 1;
+    constexpr float A_UNIT = INT4 && PRECISE && !BF ? 8.0f : 1.0f;  // of the first operand (dequant8)
     constexpr uint32_t GROUPS = 3;  // of dequantising or loading warps
     constexpr uint32_t FEATURES = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
     extern __shared__ uint8_t smem_raw[];
@@ -1037,12 +1068,12 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
             uint8_t *a = smem + (size_t)to.slot * stage_bytes;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                const Scale<BF> scale(sc[g]);
+                const Scale<BF, PRECISE> scale(sc[g]);
                 const uint32_t w[4] = {q[g].x, q[g].y, q[g].z, q[g].w};
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     uint32_t v[4], l[4];
-                    dequant8<PRECISE>(w[c], scale, v, l);
+                    dequant8(w[c], scale, v, l);
                     uint8_t *o = a + (mine ^ ((g * 4 + c) << 4));
                     *reinterpret_cast<uint4 *>(o) = make_uint4(v[0], v[1], v[2], v[3]);
                     if (PRECISE)
@@ -1163,7 +1194,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
                         __syncwarp();
                         tmem_ld16(ta + j0, v);
 #pragma unroll
-                        for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
+                        for (int j = 0; j < 16; j++) sum[i][j] += A_UNIT * __uint_as_float(v[j]);
                         if (two || A_PARTS == 2) {
                             tmem_ld16(ta + u.tmem_stride + j0, v);
 #pragma unroll

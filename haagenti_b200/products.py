@@ -257,7 +257,9 @@ def linear(x, weight, bias=None, activation: int = ACT_NONE, gate=None, residual
     ``activation`` one of the ACT_ constants; ``gate`` (rows, out_features) of
     x's type; ``residual`` of the output's type, which is x's by default.
     ``out`` may be ``gate`` or ``residual`` itself.  Sums are held in f32 and
-    the result rounded once; ``out_dtype=F32`` also keeps INT4 weights exact.
+    the result rounded once.  ``out_dtype=F32`` keeps INT4 weights exact; a
+    16-bit output of more than 16 rows rounds them to x's type, as ``decode``
+    does.
     There is no backward pass: tensors that require a gradient are refused
     while autograd records."""
     return _product(x, weight, None, bias, activation, gate, residual, out_dtype, out, stream)

@@ -772,3 +772,67 @@ def test_infinite_inputs_give_what_the_definition_gives(hb, dev, form, dt, out, 
     assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
     keep = [i for i in range(m) if i not in (1, 2, 3)]
     check(got[keep], want[keep], tol[keep])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("m", [16, 64])
+def test_f32_outputs_hold_every_int4_weight(hb, dev, dt, m):
+    """A row of x that is 1 in one place gives that column of the weights, to the last bit, for
+    finite scales of every size (8 x 65504 among them) and either sign."""
+    n, k = 4096, 64
+    g = torch.Generator(device=dev).manual_seed(7)
+    nib = torch.randint(0, 256, (n * k // 2,), dtype=torch.uint8, device=dev, generator=g)
+    bits = torch.randint(0, 0x7c00, (n * k // 32,), device=dev, generator=g, dtype=torch.int32)
+    bits[:64] = torch.arange(64, device=dev)  # zero and the smallest subnormal scales
+    bits[64:96] = 0x7bff - torch.arange(32, device=dev)
+    bits[96:128] = 0x1bf0 + torch.arange(32, device=dev)  # about 2^-8
+    sign = torch.randint(0, 2, (n * k // 32,), device=dev, generator=g, dtype=torch.int32)
+    scales = torch.where(sign > 0, bits - 32768, bits).to(torch.int16).view(torch.float16)
+    data = torch.cat([scales.view(torch.uint8), nib])
+    x = torch.eye(k, device=dev)[:m].to(DT[dt])
+    got = hb.linear(x, hb.Int4Weight(data, n, k), out_dtype=hb.F32)
+    assert torch.equal(got, weight64(data, n, k).float().t()[:m])
+    off = torch.tensor([0, m], dtype=torch.int32, device=dev)
+    got = hb.grouped_linear(x, hb.Int4Weight([data], n, k), off, out_dtype=hb.F32)
+    assert torch.equal(got, weight64(data, n, k).float().t()[:m])
+
+
+@pytest.mark.parametrize("m", [1, 12, 16, 17, 40, 150, 300])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_int4_weights_past_the_range_of_f16(hb, dev, m, out):
+    """fp16 x and finite scales whose weights pass 65504: exact for F32 outputs and up to 16 rows;
+    else such weights are infinite, as their decoded form is."""
+    n, k = 160, 320
+    g = torch.Generator(device=dev).manual_seed(m)
+    s = torch.full((n * k // 32,), 0.01, dtype=torch.float16, device=dev)
+    s[::7], s[3] = 9000.0, 65504.0
+    nib = torch.randint(0, 256, (n * k // 2,), dtype=torch.uint8, device=dev, generator=g)
+    data = torch.cat([s.view(torch.uint8), nib])
+    x = (1e-3 * torch.randn(m, k, device=dev, generator=g)).to(torch.float16)
+    got = hb.linear(x, hb.Int4Weight(data, n, k), out_dtype=TAG[out])
+    w = weight64(data, n, k)
+    if out == "f32" or m <= 16:
+        want, tol = define(x, w, None, 0, None, None, DT[out], False)
+        check(got, want, tol)
+    else:
+        r = w.to(torch.float16).double()
+        want, tol = define(x, r, None, 0, None, None, DT[out], False)
+        fine = want.isfinite()
+        assert torch.equal(got.isfinite(), fine) and torch.equal(got.isnan(), want.isnan())
+        check(torch.where(fine, got.double(), 0), torch.where(fine, want, 0), torch.where(fine, tol, 0))
+
+
+@pytest.mark.parametrize("form", ["int4", "dense"])
+@pytest.mark.parametrize("m", [16, 17, 150])
+@pytest.mark.parametrize("k", [1024, 8192])
+def test_f32_output_of_f16_keeps_its_precision(hb, dev, form, m, k):
+    """test_f32_output_keeps_its_precision with fp16 x.  INT4: the rounded weights' section is 16
+    truncated steps, and the remainders', 2^-10 of it at most, another 16.  Weights without their
+    remainders would be off by 2e-4."""
+    n = 256
+    d = make(dev, k + 1, m, n, k, 1, form, "f16", "f32", False, False, False)
+    got = run_linear(hb, d, n, k, form, 0, "f32").double()
+    w = weight64(d["w"][0], n, k) if form == "int4" else d["w"][0].double()
+    want = d["x"].double() @ w.t()
+    rel = float((got - want).norm() / want.norm())
+    assert rel <= 16 * 2.0 ** -23 * (1 + 2.0 ** -10) * (k / 256) ** 0.5 + k / 256 * 2.0 ** -24, rel
