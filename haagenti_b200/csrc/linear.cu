@@ -2080,12 +2080,12 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     const bool x_rows = tma_rows(p.x, p.M, p.ldx, p.K);
     if (int4) {
         // the stream kernel for a few rows, and for any number of rows that TMA cannot
-        // fetch; but not for many tiles of fewer K blocks than its warps (500 rows on 59
-        // experts of 23104 x 224: 160 us here, 248 there)
+        // fetch or that are empty; but not for many tiles of fewer K blocks than its warps
+        // (500 rows on 59 experts of 23104 x 224: 160 us here, 248 there)
         const uint32_t active = std::min(p.E, p.M);
         const bool shorts = p.E > 1 && pk_kblocks(p.K) < ST_WARPS &&
                             (uint64_t)active * ((p.N + 127) / 128) > 2ull * sm_count();
-        if (!x_rows || (p.M <= STREAM_ROWS * active && !shorts)) return code_of(run_stream(p, bf, s));
+        if (!x_rows || !p.K || (p.M <= STREAM_ROWS * active && !shorts)) return code_of(run_stream(p, bf, s));
         return code_of(run_umma(p, grouped, FORM_INT4, bf, s));
     }
     const bool w_rows = tma_rows(p.w, p.N, p.ldw, p.K) &&

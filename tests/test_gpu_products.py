@@ -13,6 +13,7 @@ slope: gelu's is at most 1.13):
 
 Where the bounds add up, |gate| multiplies all but the last.
 """
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -836,3 +837,30 @@ def test_f32_output_of_f16_keeps_its_precision(hb, dev, form, m, k):
     want = d["x"].double() @ w.t()
     rel = float((got - want).norm() / want.norm())
     assert rel <= 16 * 2.0 ** -23 * (1 + 2.0 ** -10) * (k / 256) ** 0.5 + k / 256 * 2.0 ** -24, rel
+
+
+@pytest.mark.parametrize("m", [3, 16, 40, 300])
+@pytest.mark.parametrize("form", ["int4", "dense"])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_no_input_features_through_the_c_abi(hb, dev, m, form, grouped):
+    """in_features of 0 is a product of zero, whatever stands for x and the weights."""
+    L, n, e = hb._lib, 136, 2 if grouped else 1
+    bias = torch.randn(e, n, device=dev).to(torch.bfloat16)
+    gate, res = (torch.randn(m, n, device=dev).to(torch.bfloat16) for _ in range(2))
+    off = torch.tensor([0, m // 3, m], dtype=torch.int32, device=dev)
+    for out_t in ("bf16", "f32"):
+        out = torch.full((m, n), 7.0, dtype=DT[out_t], device=dev)
+        r = res.to(DT[out_t])
+        a = L.LinearArgs(rows=m, out_features=n, in_features=0, d_x=None, ldx=0, d_weight=None, ldw=0,
+                         weight_stride=0, d_bias=bias.data_ptr(), d_gate=gate.data_ptr(), ldgate=n,
+                         d_residual=r.data_ptr(), ldresidual=n, d_out=out.data_ptr(), ldout=n,
+                         d_offsets=off.data_ptr(), experts=e, offsets_bits=32, x_dtype=L.BF16,
+                         weight_form=L.WEIGHT_INT4 if form == "int4" else L.WEIGHT_DENSE,
+                         bias_dtype=L.BF16, out_dtype=TAG[out_t], activation=L.ACT_RELU, reserved=0)
+        f = L.load().hct_b200_grouped_linear if grouped else L.load().hct_b200_linear
+        assert f(C.byref(a), torch.cuda.current_stream().cuda_stream) == L.OK
+        rows = torch.arange(m, device=dev)
+        b = bias[(rows >= m // 3).long()] if grouped else bias
+        want = b.double().clamp(min=0) * gate.double() + r.double()
+        check(out, want, (U[DT[out_t]] + 2 * 2.0 ** -24) * want.abs() + 2.0 ** -23 * (b * gate).double().abs())
+    hb.linear_status()
