@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "timeouts.cuh"
 
 namespace hct {
 namespace {
@@ -226,7 +227,7 @@ __device__ __forceinline__ float bias_of(const LinParams &p, uint32_t e, uint32_
                       : from16<BF>(reinterpret_cast<const uint16_t *>(p.bias)[i]);
 }
 
-__device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has expired
+__device__ uint32_t g_linear_timeouts;  // bounded waits that have expired, never cleared
 
 // ---- tensor-core kernel ---------------------------------------------------------
 //
@@ -281,7 +282,7 @@ __device__ int g_linear_status;  // HCT_B200_ERR_TIMEOUT once a bounded wait has
 // slots), and with one issuer, whose MMAs complete in order, the step before
 // in the group has already seen every step up to its own less (slots + 3).
 //
-// Every wait is bounded; an expired one raises g_linear_status, the CTA's
+// Every wait is bounded; an expired one is counted in g_linear_timeouts, the CTA's
 // roles leave their loops, its copies and MMAs are drained (bounded) and TMEM
 // is freed.
 constexpr int BK = 64;  // 128 bytes of a row: one swizzle row
@@ -902,7 +903,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
     const uint32_t tmem = uniform(ctl->tmem_base);
     const auto aborted = [&] { return *(volatile int *)&ctl->abort != 0; };
     const auto give_up = [&] {
-        atomicExch(&g_linear_status, HCT_B200_ERR_TIMEOUT);
+        atomicAdd(&g_linear_timeouts, 1u);
         atomicExch(&ctl->abort, 1);
     };
 
@@ -1558,7 +1559,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
         }
         if (!ok) {
             // the copies in flight end before the CTA does (bounded)
-            atomicExch(&g_linear_status, HCT_B200_ERR_TIMEOUT);
+            atomicAdd(&g_linear_timeouts, 1u);
             const int go_on = 0;
             for (uint32_t s = 0; s < ST_SLOTS; s++)
                 if (kb + s * ST_WARPS < kb1)
@@ -2112,20 +2113,17 @@ int hct_b200_grouped_linear(const hct_b200_linear_args *args, void *stream) {
 }
 
 int hct_b200_linear_status(void *stream) {
+    static hct::ReportedTimeouts reported;
     const cudaStream_t s = (cudaStream_t)stream;
-    int got = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(&got, hct::g_linear_status, sizeof(int), 0,
-                                              cudaMemcpyDeviceToHost, s);
+    int dev = 0;
+    uint32_t count = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess)
+        e = cudaMemcpyFromSymbolAsync(&count, hct::g_linear_timeouts, sizeof(count), 0,
+                                      cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return hct::code_of(e);
-    if (got) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbolAsync(hct::g_linear_status, &zero, sizeof(int), 0,
-                                    cudaMemcpyHostToDevice, s);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-        if (e != cudaSuccess) return hct::code_of(e);
-    }
-    return got;
+    return reported.report(dev, count) ? HCT_B200_ERR_TIMEOUT : HCT_B200_OK;
 }
 
 size_t hct_b200_int4_weight_bytes(size_t rows, size_t cols) {

@@ -281,8 +281,10 @@ def grouped_linear(x, weight, offsets, bias=None, activation: int = ACT_NONE, ga
 
 
 def linear_status(device=None, stream=None):
-    """Synchronise and raise if a product on the device ran into a device-side
-    timeout since the last call (its output is then undefined)."""
+    """Synchronise the stream and raise if a product on the device ran into a
+    device-side timeout that no call has reported yet (its output is then
+    undefined).  Products on other streams may be running still: theirs is
+    reported by a later call."""
     torch = _torch()
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         s = stream if stream is not None else torch.cuda.current_stream()

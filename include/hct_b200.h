@@ -272,11 +272,12 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * below 2^31, row strides up to 2^30 elements.
  * The calls allocate nothing, use no context and no shared scratch, and may be
  * captured; they run on the calling thread's current device, to which the
- * pointers and the stream must belong.  A device-side wait that expires is
- * reported by hct_b200_linear_status, which synchronises `stream` and returns
- * (and clears) the current device's status of every product since its last
- * call: HCT_B200_OK or HCT_B200_ERR_TIMEOUT, after which the outputs are
- * undefined. */
+ * pointers and the stream must belong.  A device-side wait that expires leaves
+ * the call's output undefined and is reported by hct_b200_linear_status, which
+ * synchronises `stream` and returns HCT_B200_ERR_TIMEOUT if a product on the
+ * current device, on any stream, has expired that no call has reported yet,
+ * else HCT_B200_OK.  Products that `stream` does not wait for may be running
+ * still; theirs is in a later call. */
 enum {
     HCT_B200_ACT_NONE = 0,
     HCT_B200_ACT_RELU = 1,

@@ -153,3 +153,16 @@ def test_python_refuses_host_tensors():
         H.Int4Weight(b"", 4, 48)
     with pytest.raises(ValueError, match="payload"):
         H.Int4Weight([], 4, 64)
+
+
+def test_no_timeout_is_lost_or_reported_twice(tmp_path):
+    """The host side of linear_status: counts read in any order and by many threads."""
+    cxx = shutil.which("g++")
+    if not cxx:
+        pytest.skip("no C++ compiler")
+    exe = tmp_path / "timeouts"
+    subprocess.run([cxx, "-std=c++17", "-O2", "-Wall", "-pthread", "-I",
+                    os.path.join(REPO, "haagenti_b200", "csrc"),
+                    os.path.join(REPO, "tests", "timeouts_check.cpp"), "-o", str(exe)], check=True)
+    got = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert got.stdout.strip() == "ok", got.stdout
