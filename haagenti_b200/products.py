@@ -23,6 +23,7 @@ __all__ = ["Int4Weight", "linear", "grouped_linear", "linear_status"]
 _TAG: dict = {}   # torch dtype -> F32 / F16 / BF16
 _TYPE: dict = {}  # and back
 _raw_stream = None  # device index -> its current stream's cudaStream_t
+_forward_ad = None  # torch.autograd.forward_ad
 
 
 class _Args(threading.local):
@@ -40,9 +41,10 @@ _ARGS = _Args()
 
 
 def _first_call():
-    global _raw_stream
+    global _raw_stream, _forward_ad
     torch = _torch()
     L.load()
+    from torch.autograd import forward_ad as _forward_ad  # noqa: F811
     # the handle alone: torch.cuda.current_stream builds a Stream object, 3 us of a call's 10
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                           lambda i: torch.cuda.current_stream(i).cuda_stream)
@@ -213,6 +215,12 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
     if grads and torch.is_grad_enabled():
         raise Unsupported(L.UNSUPPORTED, "the products have no backward pass: detach the tensors "
                                          "or call under torch.no_grad()")
+    # dual tensors exist within a dual level alone (one attribute read elsewhere)
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        for t in (x, wt, bias, gate, residual, out):
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise Unsupported(L.UNSUPPORTED, "the products have no forward-mode derivative: "
+                                                 "pass the tensors' primal parts")
     lib = L._lib
     fn = lib.hct_b200_linear if offsets is None else lib.hct_b200_grouped_linear
     here = torch.cuda.current_device() == dev
@@ -260,8 +268,8 @@ def linear(x, weight, bias=None, activation: int = ACT_NONE, gate=None, residual
     the result rounded once.  ``out_dtype=F32`` keeps INT4 weights exact; a
     16-bit output of more than 16 rows rounds them to x's type, as ``decode``
     does.
-    There is no backward pass: tensors that require a gradient are refused
-    while autograd records."""
+    There is no derivative: tensors that require a gradient are refused while
+    autograd records, and dual tensors of forward-mode differentiation always."""
     return _product(x, weight, None, bias, activation, gate, residual, out_dtype, out, stream)
 
 

@@ -864,3 +864,29 @@ def test_no_input_features_through_the_c_abi(hb, dev, m, form, grouped):
         want = b.double().clamp(min=0) * gate.double() + r.double()
         check(out, want, (U[DT[out_t]] + 2 * 2.0 ** -24) * want.abs() + 2.0 ** -23 * (b * gate).double().abs())
     hb.linear_status()
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "bias", "gate", "residual"])
+def test_dual_tensors_are_refused(hb, dev, name):
+    """A product that dropped a tangent in silence would give wrong derivatives."""
+    import torch.autograd.forward_ad as forward_ad
+
+    m, n, k = 4, 16, 32
+    kw = {"x": torch.randn(m, k, device=dev), "weight": torch.randn(n, k, device=dev),
+          "bias": torch.randn(n, device=dev), "gate": torch.randn(m, n, device=dev),
+          "residual": torch.randn(m, n, device=dev)}
+    kw = {i: t.to(torch.bfloat16) for i, t in kw.items()}
+    want = hb.linear(**kw)
+    off = torch.tensor([0, m], dtype=torch.int32, device=dev)
+    many = dict(kw, weight=kw["weight"][None], bias=kw["bias"][None])
+    with forward_ad.dual_level():
+        for f, args in ((hb.linear, kw), (hb.grouped_linear, dict(many, offsets=off))):
+            dual = dict(args)
+            dual[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+            with pytest.raises(hb.Unsupported, match="forward-mode"):
+                f(**dual)
+            with torch.no_grad(), pytest.raises(hb.Unsupported, match="forward-mode"):
+                f(**dual)
+            dual[name] = forward_ad.unpack_dual(dual[name]).primal
+            assert torch.equal(f(**dual), want)
+    assert torch.equal(hb.linear(**kw), want)
