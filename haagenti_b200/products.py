@@ -58,9 +58,10 @@ class Int4Weight:
     per expert, for ``grouped_linear``), laid out for the products.
 
     ``data`` is a payload: f16 scales, then nibbles, as a CUDA uint8 tensor or
-    host bytes; or a list of payloads.  The layout is made here, once, and the
-    stream is synchronised before the constructor returns, so that the weight
-    may be used on any stream of its device."""
+    host bytes; or a list of payloads.  ``device`` is the CUDA device of the
+    weight, the payload's or the current one by default.  The layout is made
+    here, once, and the stream is synchronised before the constructor returns,
+    so that the weight may be used on any stream of its device."""
 
     def __init__(self, data, rows: int, cols: int, device=None, stream=None):
         torch = _torch()
@@ -74,18 +75,21 @@ class Int4Weight:
                              "of 32 and rows positive")
         if not parts:
             raise ValueError("an INT4 weight needs a payload")
+        if device is not None:
+            device = torch.device(device)
+            if device.type != "cuda":
+                raise ValueError(f"an INT4 weight is on a CUDA device, not on {device}")
+            if device.index is None:  # the payload's, or the current one
+                device = None
         for p in parts:
             if hasattr(p, "is_cuda") and p.is_cuda:
                 if p.dtype != torch.uint8 or p.dim() != 1 or not p.is_contiguous():
                     raise ValueError("an INT4 payload is a contiguous 1-D uint8 tensor")
                 if device is None:
                     device = p.device
-                elif p.device != torch.device(device):
+                elif p.device != device:
                     raise ValueError("the payloads of one weight are on one device")
         if device is None:
-            device = torch.device("cuda", torch.cuda.current_device())
-        device = torch.device(device)
-        if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         if stream is not None and stream.device != device:
             raise ValueError(f"the stream belongs to {stream.device}, the weight to {device}")

@@ -890,3 +890,18 @@ def test_dual_tensors_are_refused(hb, dev, name):
             dual[name] = forward_ad.unpack_dual(dual[name]).primal
             assert torch.equal(f(**dual), want)
     assert torch.equal(hb.linear(**kw), want)
+
+
+def test_int4_weight_on_a_device_by_name(hb, dev):
+    """"cuda" without an index is the payload's device, or the current one."""
+    n, k = 16, 64
+    data = payload_of(torch.randn(n, k, device=dev))
+    x = torch.randn(3, k, device=dev).to(torch.float16)
+    want = hb.linear(x, hb.Int4Weight(data, n, k))
+    host = data.cpu().numpy().tobytes()
+    for payload in (data, host):
+        for name in (None, "cuda", "cuda:0", 0, torch.device("cuda"), dev):
+            w = hb.Int4Weight(payload, n, k, device=name)
+            assert w.device == w.packed.device == dev
+            assert torch.equal(hb.linear(x, w), want)
+            assert hb.Int4Weight([payload, payload], n, k, device=name).shape == (2, n, k)

@@ -166,3 +166,11 @@ def test_no_timeout_is_lost_or_reported_twice(tmp_path):
                     os.path.join(REPO, "tests", "timeouts_check.cpp"), "-o", str(exe)], check=True)
     got = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert got.stdout.strip() == "ok", got.stdout
+
+
+def test_int4_weight_is_on_a_cuda_device():
+    import haagenti_b200 as H
+
+    for payload in (bytes(4 * 64 * 9 // 16), [bytes(4 * 64 * 9 // 16)]):
+        with pytest.raises(ValueError, match="CUDA device"):
+            H.Int4Weight(payload, 4, 64, device="cpu")
