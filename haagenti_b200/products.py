@@ -48,8 +48,9 @@ def _first_call():
     # the handle alone: torch.cuda.current_stream builds a Stream object, 3 us of a call's 10
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                           lambda i: torch.cuda.current_stream(i).cuda_stream)
-    _TAG.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    _TYPE.update({v: k for k, v in _TAG.items()})
+    tags = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    _TYPE.update({v: k for k, v in tags.items()})
+    _TAG.update(tags)  # last, and at once: it tells other threads that all is set
 
 
 class Int4Weight:

@@ -174,3 +174,21 @@ def test_int4_weight_is_on_a_cuda_device():
     for payload in (bytes(4 * 64 * 9 // 16), [bytes(4 * 64 * 9 // 16)]):
         with pytest.raises(ValueError, match="CUDA device"):
             H.Int4Weight(payload, 4, 64, device="cpu")
+
+
+def test_first_call_is_complete_before_other_threads_see_it(monkeypatch):
+    """A call goes ahead once _TAG is filled: everything else that it needs is set by then."""
+    from haagenti_b200 import products as P
+
+    class Watched(dict):
+        def update(self, *a):
+            assert set(P._TYPE) == {0, 1, 2} and callable(P._raw_stream) and P._forward_ad and L._lib
+            assert not self
+            super().update(*a)
+
+    monkeypatch.setattr(P, "_TAG", Watched())
+    monkeypatch.setattr(P, "_TYPE", {})
+    monkeypatch.setattr(P, "_raw_stream", None)
+    monkeypatch.setattr(P, "_forward_ad", None)
+    P._first_call()
+    assert sorted(P._TAG.values()) == [0, 1, 2] and {P._TYPE[v] for v in P._TAG.values()} == set(P._TAG)
