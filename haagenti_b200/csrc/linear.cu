@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "per_device.cuh"
 #include "timeouts.cuh"
 
 namespace hct {
@@ -1648,16 +1649,18 @@ int code_of(cudaError_t e) {
     return HCT_B200_ERR_CUDA;
 }
 
-int sm_count() {
-    static int n = 0;
-    if (!n) {
-        int dev = 0, c = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess ||
-            cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || c <= 0)
-            c = 148;
-        n = c;
-    }
-    return n;
+// SMs of the current device.
+uint32_t sm_count() {
+    static PerDevice known;
+    int dev = -1;
+    cudaGetDevice(&dev);
+    const uint32_t n = known.get(dev, [dev] {
+        int c = 0;
+        return cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && c > 0
+                   ? (uint32_t)c
+                   : 0u;
+    });
+    return n ? n : 148;
 }
 
 // A matrix in memory: rows of `width` bytes, `stride` bytes apart.
@@ -1828,28 +1831,27 @@ cudaError_t launch_umma(const CUtensorMap &tx, const CUtensorMap &tw, const Umma
 // has room for whole ones only (clusters of 8: 8 to 16 of 18).  Asked once for
 // each device and size.
 uint32_t clusters_at_once(uint32_t size) {
-    static std::atomic<uint32_t> known[64][9];
+    static PerDevice known[9];
     int dev = 0;
     if (size < 2 || cudaGetDevice(&dev) != cudaSuccess) return 0xffffffffu;
-    std::atomic<uint32_t> *const k = dev < 64 ? &known[dev][size] : nullptr;
-    if (k && k->load(std::memory_order_relaxed)) return k->load(std::memory_order_relaxed);
-    const auto kernel = linear_umma_kernel<FORM_DENSE, true, false, false>;
-    int n = 0;
-    cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(size);
-    c.blockDim = dim3(umma_threads(FORM_DENSE));
-    c.dynamicSmemBytes = SMEM_MIN;
-    c.attrs = attr;
-    c.numAttrs = launch_attributes(attr, size);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT) !=
-            cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, kernel, &c) != cudaSuccess || n < 1) {
-        cudaGetLastError();
-        n = 1;
-    }
-    if (k) k->store((uint32_t)n, std::memory_order_relaxed);
-    return (uint32_t)n;
+    return known[size].get(dev, [size] {
+        const auto kernel = linear_umma_kernel<FORM_DENSE, true, false, false>;
+        int n = 0;
+        cudaLaunchAttribute attr[2];
+        cudaLaunchConfig_t c = {};
+        c.gridDim = dim3(size);
+        c.blockDim = dim3(umma_threads(FORM_DENSE));
+        c.dynamicSmemBytes = SMEM_MIN;
+        c.attrs = attr;
+        c.numAttrs = launch_attributes(attr, size);
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT) !=
+                cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &c) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 1;
+        }
+        return (uint32_t)n;
+    });
 }
 
 // CTAs to a tile: the K range is split over a cluster where tiles leave half of
@@ -1884,7 +1886,7 @@ uint32_t pair_rows(uint32_t M, uint32_t nt, uint32_t pairs, uint32_t cap) {
 cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaStream_t s) {
     const bool int4 = form == FORM_INT4, any = form >= FORM_ANY;
     const bool precise = p.odt == HCT_B200_F32;
-    const uint32_t sms = (uint32_t)sm_count(), cap = max_rows(form, precise);
+    const uint32_t sms = sm_count(), cap = max_rows(form, precise);
     const uint32_t kbs = std::max((p.K + BK - 1) / BK, 1u);
     const uint32_t active = std::min(p.E, p.M), per_expert = p.M / active;
     UmmaParams u{};
@@ -2023,7 +2025,7 @@ cudaError_t launch_stream(const StreamParams &q, uint32_t grid, cudaStream_t s) 
 constexpr uint32_t STREAM_ROWS = 16;  // rows (per expert with rows) up to which the stream kernel is taken
 
 cudaError_t run_stream(const LinParams &p, bool bf, cudaStream_t s) {
-    const uint32_t sms = (uint32_t)sm_count(), kbs = (uint32_t)pk_kblocks(p.K);
+    const uint32_t sms = sm_count(), kbs = (uint32_t)pk_kblocks(p.K);
     const uint32_t active = std::min(p.E, p.M);
     const bool two = p.M / active > 8 || (p.E == 1 && p.M > 8);
     StreamParams q{};

@@ -155,17 +155,27 @@ def test_python_refuses_host_tensors():
         H.Int4Weight([], 4, 64)
 
 
-def test_no_timeout_is_lost_or_reported_twice(tmp_path):
-    """The host side of linear_status: counts read in any order and by many threads."""
+def run_host_check(tmp_path, name):
     cxx = shutil.which("g++")
     if not cxx:
         pytest.skip("no C++ compiler")
-    exe = tmp_path / "timeouts"
+    exe = tmp_path / name
     subprocess.run([cxx, "-std=c++17", "-O2", "-Wall", "-pthread", "-I",
                     os.path.join(REPO, "haagenti_b200", "csrc"),
-                    os.path.join(REPO, "tests", "timeouts_check.cpp"), "-o", str(exe)], check=True)
+                    os.path.join(REPO, "tests", name + ".cpp"), "-o", str(exe)], check=True)
     got = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert got.stdout.strip() == "ok", got.stdout
+
+
+def test_no_timeout_is_lost_or_reported_twice(tmp_path):
+    """The host side of linear_status: counts read in any order and by many threads."""
+    run_host_check(tmp_path, "timeouts_check")
+
+
+def test_properties_are_each_devices_own(tmp_path):
+    """What plans ask of a device (its SMs, its clusters): no other device's, no failure remembered,
+    from many threads at once."""
+    run_host_check(tmp_path, "per_device_check")
 
 
 def test_int4_weight_is_on_a_cuda_device():
