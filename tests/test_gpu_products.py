@@ -905,3 +905,28 @@ def test_int4_weight_on_a_device_by_name(hb, dev):
             assert w.device == w.packed.device == dev
             assert torch.equal(hb.linear(x, w), want)
             assert hb.Int4Weight([payload, payload], n, k, device=name).shape == (2, n, k)
+
+
+@pytest.mark.parametrize("form", ["int4", "dense"])
+@pytest.mark.parametrize("m,n,k", [(2048, 9728, 512), (300, 19000, 1024), (1030, 4900, 2048)])
+def test_pairs_give_the_same_bits_every_time(hb, dev, form, m, n, k):
+    """Tiles that two CTAs share, one issuing for both, linear and grouped, weights of their own
+    before each call so that a K step taken too early would show."""
+    d = [make(dev, 40 + i, m, n, k, 1, form, "bf16", "bf16", False, False, False) for i in range(2)]
+    ws = [hb.Int4Weight(i["w"][0], n, k) if form == "int4" else i["w"][0] for i in d]
+    x = d[0]["x"]
+    rows = torch.tensor([0, 1, m // 2, m - 1], device=dev)
+    want = []
+    for i, w in enumerate(ws):
+        want.append(hb.linear(x, w))
+        w64 = weight64(d[i]["w"][0], n, k) if form == "int4" else w
+        v, tol = define(x[rows], w64, None, 0, None, None, torch.bfloat16, form == "int4")
+        check(want[i][rows], v, tol)
+    for i in range(20):
+        assert torch.equal(hb.linear(x, ws[i % 2]), want[i % 2])
+    both = hb.Int4Weight([i["w"][0] for i in d], n, k) if form == "int4" else torch.stack(ws)
+    off = torch.tensor([0, m // 3, m], dtype=torch.int32, device=dev)
+    first = hb.grouped_linear(x, both, off)
+    for i in range(10):
+        assert torch.equal(hb.grouped_linear(x, both, off), first)
+    hb.linear_status()
