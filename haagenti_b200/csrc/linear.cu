@@ -177,9 +177,12 @@ __device__ __forceinline__ uint32_t expert_of(const uint32_t *first, uint32_t E,
 // These kernels are launched while the one before them on the stream may still
 // run (programmatic serialisation): a kernel sets itself up and waits for
 // everything before it, in every thread, before it touches global memory; and
-// it says when the kernel after it may start doing the same.  The stream kernel
-// does not say so: early CTAs of the next kernel take the room that its clusters
-// need (1 x 4096 x 4096 in a row: 9.5 us against 7.7).
+// it says when the kernel after it may start doing the same.  One thread of a CTA
+// says so for the CTA, so it is the one that has allocated TMEM: a next kernel of
+// another library that fits beside it on an SM could else take the TMEM first and
+// wait for this kernel, which waits for the TMEM.  The stream kernel does not say
+// so: early CTAs of the next kernel take the room that its clusters need (1 x 4096 x
+// 4096 in a row: 9.5 us against 7.7).
 __device__ __forceinline__ void after_previous_kernel() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
@@ -907,8 +910,8 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
     if (warp == 1) {
         tmem_alloc<PAIR>(smem_u32(&ctl->tmem_base), u.tmem_cols);
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        let_next_kernel_start();
     }
-    let_next_kernel_start();
     after_previous_kernel();
     if (warp == 2) scan_groups(p, u.tile, groups);
     __syncthreads();

@@ -930,3 +930,29 @@ def test_pairs_give_the_same_bits_every_time(hb, dev, form, m, n, k):
     for i in range(10):
         assert torch.equal(hb.grouped_linear(x, both, off), first)
     hb.linear_status()
+
+
+def test_products_among_other_kernels(hb, dev):
+    """Products between library products and the library's own decode on one stream, each of whose
+    kernels may start while the one before it ends: every result as when it runs alone."""
+    from oracle import hct as OH
+
+    m, n, k = 512, 1024, 1024
+    d = make(dev, 60, m, n, k, 1, "int4", "bf16", "bf16", False, False, False)
+    q, x = hb.Int4Weight(d["w"][0], n, k), d["x"]
+    w = weight64(d["w"][0], n, k).to(torch.bfloat16)
+    r = hb.HctReader(OH.encode_spectral_q4(OH.gen_weight((256, 512), 2)))
+    calls = [lambda: hb.linear(x, q), lambda: x @ w.t(), lambda: hb.linear(x[:40], q),
+             lambda: hb.linear(x[:4], q), lambda: r.decode(hb.BF16), lambda: hb.linear(x, w),
+             lambda: x[:64] @ w.t(), lambda: hb.linear(x, q, out_dtype=hb.F32)]
+    want = []
+    for c in calls:
+        want.append(c())
+        torch.cuda.synchronize()
+    for rep in range(10):
+        order = np.random.default_rng(rep).permutation(np.repeat(np.arange(len(calls)), 4))
+        got = [(i, calls[i]()) for i in order]
+        torch.cuda.synchronize()
+        for i, y in got:
+            assert torch.equal(y, want[i]), i
+    hb.linear_status()
