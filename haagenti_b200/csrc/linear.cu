@@ -2150,7 +2150,11 @@ int hct_b200_linear_status(void *stream) {
     const cudaStream_t s = (cudaStream_t)stream;
     int dev = 0;
     uint32_t count = 0;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaStreamIsCapturing(s, &capture);
+    // a stream that is being captured cannot be waited for: the attempt would end the capture
+    if (capture != cudaStreamCaptureStatusNone) return HCT_B200_ERR_UNSUPPORTED;
     if (e == cudaSuccess)
         e = cudaMemcpyFromSymbolAsync(&count, hct::g_linear_timeouts, sizeof(count), 0,
                                       cudaMemcpyDeviceToHost, s);

@@ -277,7 +277,8 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * synchronises `stream` and returns HCT_B200_ERR_TIMEOUT if a product on the
  * current device, on any stream, has expired that no call has reported yet,
  * else HCT_B200_OK.  Products that `stream` does not wait for may be running
- * still; theirs is in a later call. */
+ * still; theirs is in a later call.  A stream that is being captured is
+ * HCT_B200_ERR_UNSUPPORTED. */
 enum {
     HCT_B200_ACT_NONE = 0,
     HCT_B200_ACT_RELU = 1,

@@ -956,3 +956,20 @@ def test_products_among_other_kernels(hb, dev):
         for i, y in got:
             assert torch.equal(y, want[i]), i
     hb.linear_status()
+
+
+def test_status_does_not_end_a_capture(hb, dev):
+    """linear_status on a stream that is being captured is refused, and the graph stays good."""
+    x, w = torch.ones(4, 64, device=dev, dtype=torch.float16), torch.ones(8, 64, device=dev, dtype=torch.float16)
+    hb.linear(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = hb.linear(x, w)
+        with pytest.raises(hb.Unsupported):
+            hb.linear_status()
+        z = hb.linear(x, w, residual=y)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (y == 64).all() and (z == 128).all()
+    hb.linear_status()
