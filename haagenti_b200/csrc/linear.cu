@@ -1431,14 +1431,19 @@ __device__ __forceinline__ void mma_more(float (&d)[4], uint32_t a0, uint32_t a1
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The pairs of a word as nibble - 8 in x's type (see dequant8).
+// The pairs of a word as nibble - 8 in x's type (see dequant8), in bf16 times 2^-8
+// (ST_UNIT): 32 products of x's largest value are then within f32, as its products
+// with the weights are.
+template <bool BF>
+constexpr float ST_UNIT = BF ? 256.0f : 1.0f;
 template <bool BF>
 __device__ __forceinline__ void nibbles8(uint32_t w, uint32_t (&v)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if (BF) {
             uint32_t b = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
-            v[j] = bits_of(__hsub2(*reinterpret_cast<__nv_bfloat162 *>(&b), __float2bfloat162_rn(136.0f)));
+            v[j] = bits_of(__hfma2(*reinterpret_cast<__nv_bfloat162 *>(&b), __float2bfloat162_rn(0.00390625f),
+                                   __float2bfloat162_rn(-0.53125f)));
         } else {
             uint32_t b = (j & 1 ? (w >> (8 * (j / 2))) & 0x00f000f0u
                                 : (w >> (8 * (j / 2))) & 0x000f000fu) | 0x64006400u;
@@ -1635,7 +1640,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
     }
     const auto finish = [&]() {
 #pragma unroll
-        for (int j = 0; j < 8; j++) z[j] += bias[j];
+        for (int j = 0; j < 8; j++) z[j] = fmaf(ST_UNIT<BF>, z[j], bias[j]);
         finish8<BF, OUT_ANY>(p, z, o, m0 + mine, n);
     };
     if (q.split == 1) {

@@ -973,3 +973,21 @@ def test_status_does_not_end_a_capture(hb, dev):
     torch.cuda.synchronize()
     assert (y == 64).all() and (z == 128).all()
     hb.linear_status()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("m", [1, 8, 16, 17, 60])
+def test_largest_inputs_with_int4_weights(hb, dev, dt, m):
+    """x at its type's ends times weights below 1: the products are within range, and so is every
+    step on the way to them."""
+    n, k = 160, 320
+    d = make(dev, 70 + m, m, n, k, 1, "int4", dt, "f32", False, False, False)
+    big, row = torch.finfo(DT[dt]).max, torch.arange(m, device=dev)
+    d["x"][row, row * 7 % k] = torch.where(row % 2 == 0, big, -big).to(DT[dt])
+    w = weight64(d["w"][0], n, k)
+    assert w.abs().max() < 1
+    for out in ("f32", dt):
+        want, tol = define(d["x"], w, None, 0, None, None, DT[out], True)
+        fine = want.abs() <= 0.99 * torch.finfo(DT[out]).max
+        got = run_linear(hb, d, n, k, "int4", 0, out)
+        check(torch.where(fine, got.double(), 0), torch.where(fine, want, 0), tol, out)
