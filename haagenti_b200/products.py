@@ -60,7 +60,7 @@ class Int4Weight:
 
     ``data`` is a payload: f16 scales, then nibbles, as a CUDA uint8 tensor or
     host bytes; or a list of payloads.  ``device`` is the CUDA device of the
-    weight, the payload's or the current one by default.  The layout is made
+    weight: the payload's, the stream's or the current one by default.  The layout is made
     here, once, and the stream is synchronised before the constructor returns,
     so that the weight may be used on any stream of its device."""
 
@@ -91,7 +91,8 @@ class Int4Weight:
                 elif p.device != device:
                     raise ValueError("the payloads of one weight are on one device")
         if device is None:
-            device = torch.device("cuda", torch.cuda.current_device())
+            device = (stream.device if stream is not None
+                      else torch.device("cuda", torch.cuda.current_device()))
         if stream is not None and stream.device != device:
             raise ValueError(f"the stream belongs to {stream.device}, the weight to {device}")
         with torch.cuda.device(device):
@@ -299,6 +300,8 @@ def linear_status(device=None, stream=None):
     undefined).  Products on other streams may be running still: theirs is
     reported by a later call."""
     torch = _torch()
-    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+    if device is None:
+        device = stream.device if stream is not None else torch.cuda.current_device()
+    with torch.cuda.device(device):
         s = stream if stream is not None else torch.cuda.current_stream()
         _check(L.load().hct_b200_linear_status(s.cuda_stream))

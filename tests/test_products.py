@@ -202,3 +202,41 @@ def test_first_call_is_complete_before_other_threads_see_it(monkeypatch):
     monkeypatch.setattr(P, "_forward_ad", None)
     P._first_call()
     assert sorted(P._TAG.values()) == [0, 1, 2] and {P._TYPE[v] for v in P._TAG.values()} == set(P._TAG)
+
+
+class Reached(Exception):
+    """Raised in the place of making a device current, with that device."""
+
+
+@pytest.fixture
+def two_devices(monkeypatch):
+    """torch, as products.py sees it, with device 0 current and devices that cannot be entered."""
+    import types
+
+    import torch
+
+    from haagenti_b200 import products as P
+
+    def enter(device):
+        raise Reached(torch.device("cuda", device) if isinstance(device, int) else torch.device(device))
+
+    cuda = types.SimpleNamespace(device=enter, current_device=lambda: 0)
+    fake = types.SimpleNamespace(cuda=cuda, device=torch.device, uint8=torch.uint8)
+    monkeypatch.setattr(P, "_torch", lambda: fake)
+    return P, torch, types.SimpleNamespace(device=torch.device("cuda", 1))
+
+
+def test_a_stream_names_the_device(two_devices):
+    """Where only a stream is given, its device is meant and not the current one."""
+    P, torch, stream = two_devices
+    payload = bytes(4 * 64 * 9 // 16)
+    for kw, want in (({}, 0), ({"stream": stream}, 1), ({"device": 1}, 1), ({"device": "cuda:0"}, 0),
+                     ({"device": "cuda", "stream": stream}, 1)):
+        with pytest.raises(Reached) as e:
+            P.linear_status(**{k: v for k, v in kw.items() if v != "cuda"})
+        assert e.value.args[0] == torch.device("cuda", want), kw
+        with pytest.raises(Reached) as e:
+            P.Int4Weight(payload, 4, 64, **kw)
+        assert e.value.args[0] == torch.device("cuda", want), kw
+    with pytest.raises(ValueError, match="stream belongs"):
+        P.Int4Weight(payload, 4, 64, device=0, stream=stream)
