@@ -235,9 +235,13 @@ def _product(x, weight, offsets, bias, activation, gate, residual, out_dtype, ou
             out = x.new_empty(m, n) if ot is xt else torch.empty(m, n, dtype=ot, device=x.device)
             ldo = n
         a = _ARGS
-        a.layout.pack_into(a.buffer, 0, m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride,
-                           bias_ptr, gate_ptr, ldg, res_ptr, ldr, out.data_ptr(), ldo,
-                           off_ptr, experts, bits, x_tag, form, bias_tag, tag, activation, 0)
+        try:
+            a.layout.pack_into(a.buffer, 0, m, n, k, x.data_ptr(), ldx, wt.data_ptr(), ldw, w_stride,
+                               bias_ptr, gate_ptr, ldg, res_ptr, ldr, out.data_ptr(), ldo,
+                               off_ptr, experts, bits, x_tag, form, bias_tag, tag, activation, 0)
+        except struct.error:  # every other value has been checked
+            raise ValueError("activation must be one of the ACT_ constants, "
+                             f"got {activation!r}") from None
         raw = _raw_stream(dev)
         rc = fn(a.args, raw)
         if rc:

@@ -991,3 +991,11 @@ def test_largest_inputs_with_int4_weights(hb, dev, dt, m):
         fine = want.abs() <= 0.99 * torch.finfo(DT[out]).max
         got = run_linear(hb, d, n, k, "int4", 0, out)
         check(torch.where(fine, got.double(), 0), torch.where(fine, want, 0), tol, out)
+
+
+@pytest.mark.parametrize("activation", ["silu", None, 1.0, 1 << 40, -(1 << 40)])
+def test_activations_are_constants(hb, dev, activation):
+    x, w = torch.ones(4, 64, device=dev, dtype=torch.float16), torch.ones(8, 64, device=dev, dtype=torch.float16)
+    with pytest.raises(ValueError, match="ACT_ constants"):
+        hb.linear(x, w, activation=activation)
+    assert (hb.linear(x, w) == 64).all()
