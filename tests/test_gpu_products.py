@@ -999,3 +999,41 @@ def test_activations_are_constants(hb, dev, activation):
     with pytest.raises(ValueError, match="ACT_ constants"):
         hb.linear(x, w, activation=activation)
     assert (hb.linear(x, w) == 64).all()
+
+
+@pytest.mark.parametrize("form", ["int4", "dense"])
+@pytest.mark.parametrize("m", [12, 50, 400])
+def test_descending_offsets_row_by_row(hb, dev, form, m):
+    """Every row of a call whose offsets descend, those after a descent among them: a value below
+    its predecessors counts as the largest before it."""
+    n, k, e = 96, 128, 5
+    d = make(dev, 80 + m, m, n, k, e, form, "f16", "f16", True, False, False)
+    w = hb.Int4Weight(d["w"], n, k) if form == "int4" else torch.stack(d["w"])
+    for offsets in ([-5, m // 3, 1, m // 2, 0, 1 << 30], [2, m // 2, m // 4, m // 4, m - 1, 0],
+                    [m // 3, 0, 0, 0, m // 2, m // 4]):
+        ends = np.maximum.accumulate(np.clip(offsets, 0, m))
+        y = torch.full((m, n), 7.0, dtype=torch.float16, device=dev)
+        off = torch.tensor(offsets, dtype=torch.int32, device=dev)
+        hb.grouped_linear(d["x"], w, off, d["bias"], out=y)
+        assert (y[:ends[0]] == 7).all() and (y[ends[-1]:] == 7).all()
+        for i in range(e):
+            q = slice(int(ends[i]), int(ends[i + 1]))
+            wi = weight64(d["w"][i], n, k) if form == "int4" else d["w"][i]
+            want, tol = define(d["x"][q], wi, d["bias"][i], 0, None, None, torch.float16, form == "int4")
+            check(y[q], want, tol, (offsets, i))
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_experts_interleaved_or_shared(hb, dev, m):
+    """Expert weights whose rows lie between one another's, and one matrix for every expert."""
+    n, k, e = 96, 128, 4
+    g = torch.Generator(device=dev).manual_seed(m)
+    x = torch.randn(m, k, device=dev, generator=g).to(torch.bfloat16)
+    rows = torch.randn(n, e, k, device=dev, generator=g).to(torch.bfloat16)
+    off = torch.tensor([0, m // 4, m // 4, m // 2, m], dtype=torch.int64, device=dev)
+    for w in (rows.transpose(0, 1), rows[:, 0].expand(e, n, k), rows[:, 1].contiguous().expand(e, n, k)):
+        y = hb.grouped_linear(x, w, off)
+        for i in range(e):
+            q = slice(int(off[i]), int(off[i + 1]))
+            want, tol = define(x[q], w[i], None, 0, None, None, torch.bfloat16, False)
+            check(y[q], want, tol, i)
