@@ -182,7 +182,7 @@ __device__ __forceinline__ uint32_t expert_of(const uint32_t *first, uint32_t E,
 // another library that fits beside it on an SM could else take the TMEM first and
 // wait for this kernel, which waits for the TMEM.  The stream kernel does not say
 // so: early CTAs of the next kernel take the room that its clusters need (1 x 4096 x
-// 4096 in a row: 9.5 us against 7.7).
+// 4096 in a row: 7.1 us against 6.8).
 __device__ __forceinline__ void after_previous_kernel() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
@@ -267,9 +267,9 @@ __device__ uint32_t g_linear_timeouts;  // bounded waits that have expired, neve
 // accumulators are double-buffered, so a tile's epilogue runs under the next
 // tile's MMAs.  With fewer, the K range of a tile is split over a cluster of
 // CTAs: each pushes the rows that another finishes into that one's shared memory
-// by bulk copies (reading them there took 6 to 8 bytes a clock: 196 x 1792 x 1664
-// 17.6 us, pushed 9.6), and a row's parts are added in rank order: no workspace,
-// no atomics, the same bits every time.
+// by bulk copies (196 x 1792 x 1664: 9.4 us; reading them there with
+// ld.shared::cluster, 6 to 8 bytes a clock, took 17.6), and a row's parts are added
+// in rank order: no workspace, no atomics, the same bits every time.
 //
 // F32 outputs (PRECISE) accumulate at most SECTION K steps in TMEM and add the
 // sections in registers with rounding; INT4 weights are then two A operands,
@@ -292,7 +292,7 @@ __device__ uint32_t g_linear_timeouts;  // bounded waits that have expired, neve
 constexpr int BK = 64;  // 128 bytes of a row: one swizzle row
 constexpr int A_BYTES = 128 * BK * 2;
 constexpr int MAX_STAGES = 8, MAX_RAW = 16;
-constexpr int SECTION = 4;  // 256 products: at most 16 truncated sums
+constexpr int SECTION = 4;  // 256 products to an accumulator: at most 16 truncated sums
 constexpr uint32_t SMEM_LIMIT = 232448;  // 227 KB
 constexpr uint32_t SMEM_MIN = 120 * 1024;  // one CTA per SM: TMEM is never waited for
 constexpr uint32_t RASTER = 8;
@@ -588,7 +588,10 @@ __device__ __forceinline__ Tile tile_at(const UmmaParams &u, const Groups &g, ui
 }
 
 // Eight INT4 values times their scale as four pairs of x's type, and for
-// PRECISE what the rounding of each left.
+// PRECISE what the rounding of each left.  Without PRECISE the rounding stays in the
+// result of a 16-bit output, as it does when a weight is decoded to x's type: in
+// bf16 2.4e-3 of the norm against 1.7e-3 with the output rounded alone.  Two operands
+// for every output would double the MMAs.
 //
 // (word >> 4 j) & 0x000f000f are the nibbles of the pair (2 j, 2 j + 1); or'ed
 // into the mantissa of 1024 (fp16) or 128 (bf16) they are 1024 + n or 128 + n
@@ -994,8 +997,8 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
         const uint32_t full = smem_u32(ANY || (INT4 && (lane & 8u)) ? ctl->afull : ctl->xfull);
         // INT4: two steps to a wait where that leaves the ring three to be filled
         // meanwhile.  The issuing warp shares its scheduler with three dequantising
-        // ones; 2048 x 14336 x 4096 takes 192 us for 203.  Dense operands, which come
-        // in order from one producer, lose by it (170 us for 168)
+        // ones; 2048 x 14336 x 4096 with SiLU and gate takes 190 us for 213.  Dense
+        // operands, which come in order from one producer, lost by it (170 us for 168)
         const bool pairs = INT4 && u.issuers == 1 && stages >= 5;
         const uint32_t me = warp - 1, every = u.issuers - 1;  // slots: me modulo u.issuers
         Ring at(stages), acc(2);
@@ -1287,8 +1290,7 @@ __global__ void __launch_bounds__(umma_threads(FORM), 1)
     if (!PAIR && u.split > 1) {
         // one tile per cluster: each CTA finishes its share of the tile's rows, adding the
         // CTAs' parts in rank order.  A CTA pushes every other one its rows by one bulk
-        // copy (reading them there with ld.shared::cluster moved 6 to 8 bytes a clock: 10
-        // us for 196 rows).  The barriers and the wait are reached on every path
+        // copy.  The barriers and the wait are reached on every path
         constexpr int OUT = PRECISE ? OUT_F32 : OUT_16;
         Tile c{};
         uint32_t j = 0, j0 = 0, j1 = 0, n = 0;
@@ -1961,7 +1963,7 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     };
     // Clocks of a plan, roughly: a K step takes its MMAs (2 a row), its issuing (300 with
     // two issuers, else 550; INT4 550), its bytes from L2 (50 a clock to an SM) or the copies
-    // of its rows by warps (17 each, 11 in words; 4096 x 4096 x 1001 217 us, K = 1004 143), and
+    // of its rows by warps (17 each, 11 in words; 4096 x 4096 x 1001 216 us, K = 1002 142), and
     // a split 2500 more and 40 for a row of its tile that is sent.
     const auto clocks = [&] {
         const uint32_t bytes = (int4 ? PK_BYTES : (uint32_t)A_BYTES) + u.bn * 128;
@@ -1973,10 +1975,10 @@ cudaError_t run_umma(const LinParams &p, bool grouped, int form, bool bf, cudaSt
     if (pair) {
         plan(grouped ? cap : pair_rows(p.M, nt, sms / 2, cap));
     } else {
-        // Lower tiles may use more SMs (196 x 1792 x 1664: 112 rows and 5 parts of K 9.9
-        // us, 208 rows and 4 parts 11.6) or not (256 x 8192 x 8192 INT4: 256 rows and 2
-        // parts 40 us, 128 rows 65).  linear: M in up to 6 tiles more than it needs,
-        // of 48 rows or more (16 where copying bounds: 80 x 64 x 12511 39 us, 45 in one tile);
+        // Lower tiles may use more SMs (196 x 1792 x 1664: 48 rows and 2 parts of K 9.4
+        // us, 208 rows and 4 parts 13.6) or not (256 x 8192 x 8192 INT4: 256 rows and 2
+        // parts 43 us, 128 rows 56).  linear: M in up to 6 tiles more than it needs,
+        // of 48 rows or more (16 where copying bounds: 80 x 64 x 12511 40 us, 53 in one tile);
         // grouped, whose groups are not known here: some heights
         uint32_t best = 0;
         uint64_t least = ~0ull;
@@ -2120,7 +2122,7 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     if (int4) {
         // the stream kernel for a few rows, and for any number of rows that TMA cannot
         // fetch or that are empty; but not for many tiles of fewer K blocks than its warps
-        // (500 rows on 59 experts of 23104 x 224: 160 us here, 248 there)
+        // (500 rows on 59 experts of 23104 x 224: 165 us here, 223 there)
         const uint32_t active = std::min(p.E, p.M);
         const bool shorts = p.E > 1 && pk_kblocks(p.K) < ST_WARPS &&
                             (uint64_t)active * ((p.N + 127) / 128) > 2ull * sm_count();
@@ -2130,7 +2132,7 @@ int run(const hct_b200_linear_args *a, bool grouped, cudaStream_t s) {
     const bool w_rows = tma_rows(p.w, p.N, p.ldw, p.K) &&
                         (p.E == 1 || (p.w_stride % 8 == 0 && p.w_stride && p.w_stride < 1ull << 38));
     if (p.K && x_rows && w_rows) return code_of(run_umma(p, grouped, FORM_DENSE, bf, s));
-    // rows that TMA cannot fetch (500 x 5000 x 4002: 129 us with loads of 4 bytes, 203 of 2)
+    // rows that TMA cannot fetch (500 x 5000 x 4002: 114 us with loads of 4 bytes, 195 of 2)
     const bool words = ((uintptr_t)p.x | (uintptr_t)p.w) % 4 == 0 && p.K % 2 == 0 &&
                        (p.M == 1 || p.ldx % 2 == 0) && (p.N == 1 || p.ldw % 2 == 0) &&
                        (p.E == 1 || p.w_stride % 2 == 0);

@@ -263,8 +263,11 @@ int hct_b200_dequantize_int4_mp(const uint8_t *d_data, size_t data_len, size_t n
  * experts with in_features up to 448, which round them too.
  *
  * Strides are in elements.  Rows of x and w that start on 16-byte boundaries
- * are fetched by TMA; others are copied by plain loads, several times slower
- * (4-byte loads where rows start on 4 bytes and in_features is even).  out may
+ * are fetched by TMA; others are copied by plain loads, four to six times slower
+ * (4-byte loads where rows start on 4 bytes and in_features is even).  An INT4
+ * product with such an x reads the weights once for every 16 of its rows (2048 of
+ * them: nine times slower).  A block of INT4 weights whose scale is infinite or NaN
+ * gives values that are not finite.  out may
  * be the same matrix as gate or residual (same pointer, stride and type); any
  * other overlap of out with an input is HCT_B200_ERR_INVALID_ARGUMENT, as are
  * out rows that overlap one another.  rows == 0 or out_features == 0 is a
